@@ -49,7 +49,7 @@ def listed():
         # One decode step of 64 sequences: K rotated, K and V quantised into their pages.
         {"name": "append 64", "op": "append", "B": 64, "lo": 100, "hi": 1000, "Hkv": 8, "D": 128, "R": 128, "page": 16,
          "fp8": True, "interleaved": False},
-        # A 2048-token chunk written behind a 30720-token prefix, the whole prefix read back for the chunk's attention.
+        # A 2048-token chunk written at the end of a 32768-token sequence, all of it read back for the chunk's attention.
         {"name": "chunk 2k at 30k", "op": "chunk", "B": 1, "n": 2048, "lo": 32768, "hi": 32768, "Hkv": 8, "D": 128,
          "R": 128, "page": 64, "fp8": True, "interleaved": False},
         # Ragged chunks of 5 sequences in 8-token pages, heads of 64, half of the head rotated; the bf16 cache.
