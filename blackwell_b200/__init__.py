@@ -10,3 +10,6 @@ from .attention import (  # noqa: F401
     lse_combine, qk_norm_rope, gqa_fused_fwd, sdpa_gqa, sdpa_gqa_causal, stream_status, set_option, get_option,
     shard_plan, decode_workspace_size, attention_from_host, host_workspace_size, mha_fwd_f32,
 )
+from .cache import (  # noqa: F401
+    rope_table, rope, kv_cache_write, kv_cache_read, gqa_decode_paged_fp8, decode_fp8_workspace_size,
+)

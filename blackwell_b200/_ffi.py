@@ -11,7 +11,9 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libbw_attn.so"
 
-BW_OK, BW_ERR_SHAPE, BW_ERR_ALIGN, BW_ERR_CUDA, BW_ERR_TIMEOUT, BW_ERR_NCCL, BW_ERR_NULL, BW_ERR_WORKSPACE = range(8)
+(BW_OK, BW_ERR_SHAPE, BW_ERR_ALIGN, BW_ERR_CUDA, BW_ERR_TIMEOUT, BW_ERR_NCCL, BW_ERR_NULL, BW_ERR_WORKSPACE,
+ BW_ERR_INDEX) = range(9)
+BW_BF16, BW_F32, BW_E4M3 = 0, 1, 2
 BW_LAYOUT_BHSD, BW_LAYOUT_BSHD = 0, 1
 BW_OPT_TIMEOUT_NS, BW_OPT_P_IN_TMEM, BW_OPT_DEBUG_FLAGS, BW_OPT_MAX_CTAS, BW_OPT_EXP_POLY, BW_OPT_PREFILL_KERNEL = 1, 2, 3, 4, 5, 6
 
@@ -22,6 +24,12 @@ _vp, _i, _i64, _f, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c
 class BwStrides(ctypes.Structure):
     _fields_ = [("q", ctypes.c_int64 * 3), ("k", ctypes.c_int64 * 3), ("v", ctypes.c_int64 * 3),
                 ("o", ctypes.c_int64 * 3)]
+
+
+class BwRopeScaling(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int)] + [(n, ctypes.c_double) for n in (
+        "base", "factor", "original_length", "attention_factor", "beta_fast", "beta_slow", "low_freq_factor",
+        "high_freq_factor")]
 
 
 _SP = ctypes.POINTER(BwStrides)
@@ -48,6 +56,12 @@ SIGNATURES = {
     "bw_attn_fwd_host_workspace_size": (_sz, [_i, _i, _i, _i, _i]),
     "bw_attn_fwd_host": (_i, [_vp] * 5 + [_i] * 5 + [_f, _i, _i, _i, _vp, _sz, _vp]),
     "bw_gqa_fused_fwd": (_i, [_vp] * 10 + [_i] * 8 + [_f, _i, _f, _i, _vp, _sz, _vp]),
+    "bw_rope_table": (_i, [_vp, _i64, _i, _i64, _vp, _vp]),
+    "bw_rope": (_i, [_vp] * 4 + [_i] * 6 + [_vp] * 5 + [_i64, _i, _vp, _i, _i, _i, _vp]),
+    "bw_kv_cache_write": (_i, [_vp] * 4 + [_i] * 3 + [_vp] * 3 + [_i] * 3 + [_vp, _vp, _i64, _i, _vp, _i, _vp]),
+    "bw_kv_cache_read": (_i, [_vp] * 3 + [_i] * 3 + [_vp, _i, _vp, _vp, _vp] + [_i] * 3 + [_vp, _vp, _i64, _vp]),
+    "bw_gqa_decode_paged_fp8_workspace_size": (_sz, [_i] * 4),
+    "bw_gqa_decode_paged_fp8": (_i, [_vp] * 8 + [_i] * 7 + [_f, _vp, _sz, _vp]),
     "bw_stream_status": (_i, [_vp]),
     "bw_set_option": (_i, [_i, _i64]),
     "bw_get_option": (_i64, [_i]),

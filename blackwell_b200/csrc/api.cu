@@ -16,7 +16,7 @@ namespace {
 
 // Device error words: 0, or 0x100|site for a timed-out wait, 0x200 for a
 // decode workspace overflow, 0x400 for a shared-memory window the prefill
-// kernel could not align.  One word per stream (slot), so that calls on
+// kernel could not align, 0x800 for an index outside its range.  One word per stream (slot), so that calls on
 // different streams neither see nor clear each other's errors; module
 // globals are per context, so every device has its own array.  Slot 0 is
 // shared by the streams beyond the first kErrSlots - 1 distinct ones.
@@ -233,6 +233,16 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 }  // namespace
 
 namespace bw {
+
+int device_info(void* stream, int* num_sms, int** err, uint64_t* timeout_ns) {
+  DeviceState* dev = nullptr;
+  const int rc = get_device_state(&dev);
+  if (rc != BW_OK) return rc;
+  *num_sms = dev->num_sms;
+  *err = err_slot(dev, stream);
+  *timeout_ns = (uint64_t)g_timeout_ns.load();
+  return BW_OK;
+}
 
 int attn_forward(const void* Q, const void* K, const void* V, void* O, float* LSE, int B, int Hq, int Hkv, int Sq,
                  int Skv, int G, int D, float scale, int causal, const bw_strides* strides, void* stream,
@@ -660,6 +670,7 @@ int bw_stream_status(void* stream) {
   }
   if (v == 0) return BW_OK;
   if (v & 0x400) return BW_ERR_CUDA;
+  if (v & bw::kErrIndexBit) return BW_ERR_INDEX;
   if (v & 0x200) return BW_ERR_WORKSPACE;
   return BW_ERR_TIMEOUT;
 }
@@ -717,6 +728,7 @@ const char* bw_strerror(int code) {
     case BW_ERR_NCCL: return "collective failed";
     case BW_ERR_NULL: return "required pointer is NULL";
     case BW_ERR_WORKSPACE: return "workspace too small";
+    case BW_ERR_INDEX: return "index on the device out of range";
     default: return "unknown error";
   }
 }

@@ -134,6 +134,102 @@ struct NormRopeParams {
 
 cudaError_t launch_norm_rope(const NormRopeParams& p, int num_sms, cudaStream_t stream);
 
+// Bit of a stream's error word for an index that a kernel found outside its
+// range (a slot, a page, a span); the access it would have made is skipped.
+constexpr int kErrIndexBit = 0x800;
+
+// Rotary table (rope.cu): rows [first, first + length) of the cos | sin table.
+constexpr int kMaxRotaryDim = 512;
+struct RopeTableParams {
+  float* table;              // fp32 [length, R]
+  int64_t length, first;
+  int R;                     // rotary dimension (even)
+  float magnitude;           // factor on cos and sin
+  double turns[kMaxRotaryDim / 2];   // frequency of pair i in turns per position
+};
+cudaError_t launch_rope_table(const RopeTableParams& p, int num_sms, cudaStream_t stream);
+
+// Rotation of Q and, where k.H > 0, K (rope.cu): [B, H, S, D] by strides.
+struct RopeTensor {
+  const void* in;
+  void* out;
+  int64_t in_sb, in_sh, in_ss, out_sb, out_sh, out_ss;   // element strides
+  int H;
+};
+struct RopeParams {
+  RopeTensor q, k;
+  int B, S, D, R;
+  int units;                 // threads per token: R / 16 and the pass-through ones (0 in place)
+  int fp32;                  // 1: fp32 tensors, 0: bf16
+  int half;                  // 1: pairs (i, i + R/2); 0: pairs (2i, 2i + 1)
+  int inverse;
+  const float* table;        // fp32 [table_len, R]
+  int64_t table_len;
+  const int* positions;      // [B, S] or null (position = s)
+  int pos_offset;
+  int q_groups;              // set by the launch
+};
+cudaError_t launch_rope(const RopeParams& p, cudaStream_t stream);
+
+// Paged cache (kv_cache.cu): [num_pages, page_size, Hkv, D] bf16 or e4m3,
+// scales uint8 [num_pages, Hkv, 2, page_size] beside e4m3.
+struct KvWriteParams {
+  const void *k, *v;         // bf16 [T, Hkv, D] by strides
+  int64_t k_st, k_sh, v_st, v_sh;
+  void *k_cache, *v_cache;
+  uint8_t* scales;
+  const int64_t* slots;      // [T]; negative: skipped
+  int64_t num_slots;
+  int T, Hkv, D, page_size;
+  int fp8;
+  const float* table;        // null: K is not rotated
+  int64_t table_len;
+  int R, half;
+  const int* positions;      // [T]
+  int* err;
+};
+cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream);
+
+struct KvReadParams {
+  const void *k_cache, *v_cache;
+  const uint8_t* scales;
+  const int* block_table;    // [B, max_pages]
+  const int* kv_lens;        // [B] tokens to read
+  const int* kv_starts;      // [B] first token, null: 0
+  const int64_t* out_offsets;   // [B] first output row
+  void *k_out, *v_out;       // bf16 [total_rows, Hkv, D]
+  int64_t total_rows;
+  int B, Hkv, D, page_size, num_pages, max_pages;
+  int fp8;
+  int* err;
+};
+cudaError_t launch_kv_read(const KvReadParams& p, int num_sms, cudaStream_t stream);
+
+// Decode over the paged 8-bit cache (decode_fp8.cu).
+struct Fp8DecodeParams {
+  const void* Q;             // bf16 [B, Hq, D]
+  const void *k_cache, *v_cache;
+  const uint8_t* scales;
+  const int* block_table;    // [B, max_pages]
+  const int* kv_lens;        // [B]
+  void* O;                   // bf16 [B, Hq, D]
+  float* LSE;                // fp32 [B, Hq] or null
+  int B, Hq, Hkv, G, D, page_size, num_pages, max_pages;
+  int max_tokens;            // max_pages * page_size, at most 2^31 - 64
+  int groups;                // token groups; groups * Hkv blocks
+  float scale_log2;
+  float* o_part;             // [(groups + B) * Hkv, G, D] fp32
+  float* lse_part;           // [(groups + B) * Hkv, G]
+  int* prefix;               // [B + 1]
+  int* err;
+  uint64_t timeout_ns;
+};
+cudaError_t launch_decode_fp8(const Fp8DecodeParams& p, cudaStream_t stream);
+
+// What an entry point outside api.cu needs of the current device: SM count, the
+// error word of `stream`, the bound on device-side waits.  Returns a status code.
+int device_info(void* stream, int* num_sms, int** err, uint64_t* timeout_ns);
+
 // The attention forward of the C ABI with the internal extras: causal query
 // offset (multiple of 128) and LSE head stride (0 = Sq).  Returns a status code.
 int attn_forward(const void* Q, const void* K, const void* V, void* O, float* LSE, int B, int Hq, int Hkv, int Sq,

@@ -1,0 +1,210 @@
+// The paged key-value cache: new tokens' K and V written into their slots (K
+// rotated on the way, both quantised to 8 bits where the cache is 8-bit), and
+// spans of sequences read back as contiguous bf16 rows.
+//
+// Cache: [pages, page_size, Hkv, D] bf16 or e4m3; 8-bit rows have a scale byte
+// in scales [pages, Hkv, 2 (K, V), page_size] (rope_math.cuh: rows, rounding).
+// Slot = page * page_size + place in the page.
+#include <cuda_bf16.h>
+
+#include "kernels.h"
+#include "rope_math.cuh"
+
+namespace bw {
+namespace {
+
+constexpr int kThreads = 256;
+
+// Rows (token, KV head, K or V) one after the other, D / 16 lanes a row, 16
+// elements a lane: the two chunks of 8 that rotate among themselves
+// (half layout: 8 sub and R/2 + 8 sub), or 16 consecutive elements.
+template <int D, bool FP8, bool ROPE, bool HALF>
+__global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvWriteParams p) {
+  constexpr int LPR = D / 16;
+  const int64_t idx = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t rows = (int64_t)p.T * p.Hkv * 2;
+  int64_t row = idx / LPR;
+  const int sub = threadIdx.x % LPR;
+  bool live = row < rows;
+  if (!live) row = 0;   // stays for the warp's shuffles
+  const int64_t th = row >> 1;
+  const int is_v = (int)(row & 1);
+  const int64_t t = th / p.Hkv;
+  const int h = (int)(th - t * p.Hkv);
+  const int64_t slot = p.slots[t];
+  if (slot < 0) {
+    live = false;   // padding
+  } else if (slot >= p.num_slots) {
+    if (live && sub == 0) atomicCAS(p.err, 0, kErrIndexBit);
+    live = false;
+  }
+  int e0 = 16 * sub, e1 = e0 + 8;
+  bool turns = false;
+  if constexpr (ROPE) {
+    turns = !is_v && sub < (p.R >> 4);
+    if (HALF && turns) {
+      e0 = 8 * sub;
+      e1 = e0 + (p.R >> 1);
+    }
+  }
+  const __nv_bfloat16* in = static_cast<const __nv_bfloat16*>(is_v ? p.v : p.k) +
+                            (is_v ? t * p.v_st + h * p.v_sh : t * p.k_st + h * p.k_sh);
+  uint4 raw[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+  if (live) {
+    raw[0] = *reinterpret_cast<const uint4*>(in + e0);
+    raw[1] = *reinterpret_cast<const uint4*>(in + e1);
+  }
+  float x[16];
+  bf16x8_to_f32(raw[0], x);
+  bf16x8_to_f32(raw[1], x + 8);
+  if constexpr (ROPE) {
+    if (turns && live) {
+      const int64_t pos = p.positions[t];
+      if (pos >= 0 && pos < p.table_len) {
+        float c[8], sn[8];
+        const float* cs = p.table + pos * p.R + 8 * sub;
+        load8(cs, c);
+        load8(cs + (p.R >> 1), sn);
+        rotate16<HALF>(x, c, sn);
+        raw[0] = f32_to_bf16x8(x);
+        raw[1] = f32_to_bf16x8(x + 8);
+      }
+    }
+  }
+  const int64_t at = (slot * p.Hkv + h) * D;
+  if constexpr (!FP8) {
+    if (live) {
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(is_v ? p.v_cache : p.k_cache) + at;
+      *reinterpret_cast<uint4*>(out + e0) = raw[0];
+      *reinterpret_cast<uint4*>(out + e1) = raw[1];
+    }
+  } else {
+    // The row's largest finite magnitude; infinities and NaN are stored as NaN
+    // and leave the scale of the row's other elements alone.
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float a = fabsf(x[i]);
+      amax = a < INFINITY ? fmaxf(amax, a) : amax;
+    }
+#pragma unroll
+    for (int off = LPR / 2; off; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+    const int e = row_exponent(amax);
+    const float inv = pow2i(-e);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = fabsf(x[i]) < INFINITY ? x[i] * inv : __uint_as_float(0x7fffffffu);
+    if (live) {
+      uint8_t* out = static_cast<uint8_t*>(is_v ? p.v_cache : p.k_cache) + at;
+      const uint2 lo = make_uint2(f32_to_e4m3x4(x[0], x[1], x[2], x[3]), f32_to_e4m3x4(x[4], x[5], x[6], x[7]));
+      const uint2 hi = make_uint2(f32_to_e4m3x4(x[8], x[9], x[10], x[11]), f32_to_e4m3x4(x[12], x[13], x[14], x[15]));
+      *reinterpret_cast<uint2*>(out + e0) = lo;
+      *reinterpret_cast<uint2*>(out + e1) = hi;
+      if (sub == 0) {
+        const int64_t page = slot / p.page_size;
+        const int place = (int)(slot - page * p.page_size);
+        p.scales[((page * p.Hkv + h) * 2 + is_v) * p.page_size + place] = (uint8_t)(e + 127);
+      }
+    }
+  }
+}
+
+// blockIdx.y = sequence; threads walk its (token, 16-element unit of the
+// [Hkv, D] row), K and V together.
+template <int D, bool FP8>
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvReadParams p) {
+  constexpr int LPR = D / 16;
+  const int b = blockIdx.y;
+  const int len = p.kv_lens[b];
+  if (len <= 0) return;
+  const int64_t start = p.kv_starts ? p.kv_starts[b] : 0;
+  const int64_t out0 = p.out_offsets[b];
+  if (start < 0 || start + len > (int64_t)p.max_pages * p.page_size || out0 < 0 || out0 + len > p.total_rows) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(p.err, 0, kErrIndexBit);
+    return;
+  }
+  const int upr = p.Hkv * LPR;   // units a token
+  const int64_t n = (int64_t)len * upr;
+  const int* bt = p.block_table + (int64_t)b * p.max_pages;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
+    const int64_t tok = i / upr;
+    const int unit = (int)(i - tok * upr);
+    const int at = (int)(start + tok);
+    const int pi = at / p.page_size, place = at - pi * p.page_size;
+    const int page = bt[pi];
+    if (page < 0 || page >= p.num_pages) {
+      atomicCAS(p.err, 0, kErrIndexBit);
+      continue;
+    }
+    const int64_t src = ((int64_t)page * p.page_size + place) * p.Hkv * D + 16 * unit;
+    const int64_t dst = (out0 + tok) * p.Hkv * D + 16 * unit;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const void* cache = w ? p.v_cache : p.k_cache;
+      uint4* out = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(w ? p.v_out : p.k_out) + dst);
+      if constexpr (FP8) {
+        const uint4 c = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(cache) + src);
+        const int h = unit / LPR;
+        const float sc = __uint_as_float(
+            (uint32_t)p.scales[(((int64_t)page * p.Hkv + h) * 2 + w) * p.page_size + place] << 23);
+        const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
+        uint32_t o[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 a = e4m3x2_to_f32(cw[j]), d = e4m3x2_to_f32(cw[j] >> 16);
+          o[2 * j] = f32_to_bf16x2(a.x * sc, a.y * sc);
+          o[2 * j + 1] = f32_to_bf16x2(d.x * sc, d.y * sc);
+        }
+        out[0] = make_uint4(o[0], o[1], o[2], o[3]);
+        out[1] = make_uint4(o[4], o[5], o[6], o[7]);
+      } else {
+        const uint4* in = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(cache) + src);
+        const uint4 a = in[0], c = in[1];
+        out[0] = a;
+        out[1] = c;
+      }
+    }
+  }
+}
+
+template <int D, bool FP8>
+void write_launch(const KvWriteParams& p, cudaStream_t stream) {
+  const int64_t threads = (int64_t)p.T * p.Hkv * 2 * (D / 16);
+  const unsigned blocks = (unsigned)((threads + kThreads - 1) / kThreads);
+  if (p.table == nullptr) kv_write_kernel<D, FP8, false, false><<<blocks, kThreads, 0, stream>>>(p);
+  else if (p.half) kv_write_kernel<D, FP8, true, true><<<blocks, kThreads, 0, stream>>>(p);
+  else kv_write_kernel<D, FP8, true, false><<<blocks, kThreads, 0, stream>>>(p);
+}
+
+}  // namespace
+
+cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream) {
+  if (p.D == 128) {
+    if (p.fp8) write_launch<128, true>(p, stream);
+    else write_launch<128, false>(p, stream);
+  } else {
+    if (p.fp8) write_launch<64, true>(p, stream);
+    else write_launch<64, false>(p, stream);
+  }
+  return cudaGetLastError();
+}
+
+cudaError_t launch_kv_read(const KvReadParams& p, int num_sms, cudaStream_t stream) {
+  // Blocks for the longest span that the table's width or the output's rows
+  // allow, at most about 8 resident blocks' worth on every SM over all sequences.
+  int64_t most = (int64_t)p.max_pages * p.page_size;
+  if (most > p.total_rows) most = p.total_rows;
+  int64_t bx = (most * p.Hkv * (p.D / 16) + kThreads - 1) / kThreads;
+  const int64_t cap = ((int64_t)num_sms * 8 + p.B - 1) / p.B;
+  if (bx > cap) bx = cap;
+  const dim3 grid((unsigned)bx, (unsigned)p.B);
+  if (p.D == 128) {
+    if (p.fp8) kv_read_kernel<128, true><<<grid, kThreads, 0, stream>>>(p);
+    else kv_read_kernel<128, false><<<grid, kThreads, 0, stream>>>(p);
+  } else {
+    if (p.fp8) kv_read_kernel<64, true><<<grid, kThreads, 0, stream>>>(p);
+    else kv_read_kernel<64, false><<<grid, kThreads, 0, stream>>>(p);
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace bw

@@ -1,0 +1,76 @@
+// What the rotary and the cache kernels share: 16-byte conversions, the
+// rotation of 16 elements, and the 8-bit rows of the quantised cache.
+#pragma once
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+namespace bw {
+
+__device__ __forceinline__ void bf16x8_to_f32(const uint4& v, float* x) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ uint32_t f32_to_bf16x2(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+__device__ __forceinline__ uint4 f32_to_bf16x8(const float* x) {
+  return make_uint4(f32_to_bf16x2(x[0], x[1]), f32_to_bf16x2(x[2], x[3]), f32_to_bf16x2(x[4], x[5]),
+                    f32_to_bf16x2(x[6], x[7]));
+}
+__device__ __forceinline__ void load8(const float* p, float* x) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p + 4));
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+
+// Rotates 16 elements by 8 angles: pairs (i, i + 8) of the array (HALF) or
+// (2i, 2i + 1).  Each product is rounded to fp32 by itself, so that the result
+// does not depend on which product a compiler contracts into an FMA: the fused
+// write of a rotated K row and the stand-alone rotation agree to the bit.
+template <bool HALF>
+__device__ __forceinline__ void rotate16(float (&x)[16], const float (&c)[8], const float (&s)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int ia = HALF ? i : 2 * i, ib = HALF ? i + 8 : 2 * i + 1;
+    const float a = x[ia], b = x[ib];
+    x[ia] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
+    x[ib] = __fadd_rn(__fmul_rn(a, s[i]), __fmul_rn(b, c[i]));
+  }
+}
+
+// The 8-bit row: codes c = e4m3(x 2^-e), e the smallest integer with
+// max|x| <= 448 2^e.  A power of two keeps x 2^-e and c 2^e exact, so a row has
+// one rounding (half a step, 2^-4 relative, for elements within 2^14 of the
+// row's largest) and reading it back as bf16 adds none.  e is clamped to
+// [kMinExp, kMaxExp] and kept as the byte e + 127; a row of zeros has e = 0.
+// kMinExp leaves 2^-e and sums over tokens weighted with 2^e inside fp32.
+constexpr int kMinExp = -100, kMaxExp = 120;
+
+// `amax`: the largest finite magnitude of the row (>= 0).
+__device__ __forceinline__ int row_exponent(float amax) {
+  // 448 = 1.75 * 2^8: e = exponent(amax) - 8, one more where the mantissa is above 1.75
+  const int e = (int)((__float_as_uint(amax) + 0x1fffffu) >> 23) - 127 - 8;
+  return amax > 0.f ? min(max(e, kMinExp), kMaxExp) : 0;
+}
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+__device__ __forceinline__ uint32_t f32_to_e4m3x4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+// Two codes (low 16 bits) -> half2 bits; every e4m3 value is an f16 value.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xffffu), __NV_E4M3);
+  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+}
+__device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t two) {
+  const uint32_t h = e4m3x2_to_f16x2(two);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+}  // namespace bw

@@ -19,9 +19,9 @@
  *    asynchronous; they are reentrant and may be made from several host threads.
  *  - Return codes (never exit()): BW_OK, or an error below.  Argument errors are
  *    detected before any launch.  Device-side failures (a bounded wait that
- *    timed out, a workspace that was too small for the actual lengths) are
- *    recorded in the error word of the call's stream, which bw_stream_status()
- *    reads and clears.
+ *    timed out, a workspace that was too small for the actual lengths, an index
+ *    out of range) are recorded in the error word of the call's stream, which
+ *    bw_stream_status() reads and clears.
  */
 #ifndef BW_ATTN_H_
 #define BW_ATTN_H_
@@ -47,7 +47,8 @@ enum {
   BW_ERR_TIMEOUT = 4,   /* a device-side wait exceeded its bound */
   BW_ERR_NCCL = 5,      /* collective failure (multi-GPU helpers) */
   BW_ERR_NULL = 6,      /* required pointer is NULL */
-  BW_ERR_WORKSPACE = 7  /* workspace too small */
+  BW_ERR_WORKSPACE = 7, /* workspace too small */
+  BW_ERR_INDEX = 8      /* a slot, page or span given on the device is out of range */
 };
 
 /* Element strides of the batch, head and sequence axes (head-dim stride is 1). */
@@ -211,6 +212,116 @@ BW_API int bw_gqa_fused_fwd(const void* Q, const void* K, const void* V, void* O
                             int pos_offset, float eps, int interleaved, float scale, int causal, void* workspace,
                             size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Rotary positions and the paged cache, for a server around the paged decode
+ * (additions of this library: the reference has neither).
+ * ------------------------------------------------------------------------- */
+
+/* Element types. */
+enum { BW_BF16 = 0, BW_F32 = 1, BW_E4M3 = 2 };
+
+/* Frequency schedule of a rotary table.  Pair i of R / 2 turns by f_i radians
+ * per position; f_i = base^(-2i/R) for BW_ROPE_NONE, and
+ *   LINEAR  f_i / factor
+ *   NTK     f_i of the base  base * factor^(R / (R - 2))
+ *   YARN    f_i / factor * r_i + f_i * (1 - r_i),  r_i = clamp((i - lo) / (hi - lo)),
+ *           lo = max(floor(d(beta_fast)), 0), hi = min(ceil(d(beta_slow)), R - 1),
+ *           d(n) = R ln(original_length / (2 pi n)) / (2 ln base)
+ *   BANDS   f_i / factor * (1 - r_i) + f_i * r_i,
+ *           r_i = clamp((original_length f_i / 2 pi - low) / (high - low))
+ * Fields that are 0 take: beta_fast 32, beta_slow 1, low_freq_factor 1,
+ * high_freq_factor 4, attention_factor (on cos and sin) 0.1 ln(factor) + 1 for
+ * YARN with factor > 1 and else 1. */
+enum { BW_ROPE_NONE = 0, BW_ROPE_LINEAR = 1, BW_ROPE_NTK = 2, BW_ROPE_YARN = 3, BW_ROPE_BANDS = 4 };
+typedef struct bw_rope_scaling {
+  int kind;
+  double base;                 /* > 1 */
+  double factor;               /* > 0; unused by NONE */
+  double original_length;      /* > 0; YARN and BANDS */
+  double attention_factor;
+  double beta_fast, beta_slow;
+  double low_freq_factor, high_freq_factor;
+} bw_rope_scaling;
+
+/* cos | sin table fp32 [length, rotary_dim] for the positions first .. first +
+ * length - 1 (first + length <= 2^31): cos in the first half of a row, sin in
+ * the second, as bw_qk_norm_rope, bw_rope and bw_kv_cache_write read it.
+ * Angles are reduced in fp64.  rotary_dim: even, at most 512.  scaling NULL:
+ * BW_ROPE_NONE with base 10000. */
+BW_API int bw_rope_table(float* table, int64_t length, int rotary_dim, int64_t first, const bw_rope_scaling* scaling,
+                         void* stream);
+
+/* Rotates the first `rotary_dim` elements of every head of Q [B, Hq, S, D] and
+ * of K [B, Hkv, S, D] (K NULL with Hkv 0: Q alone) in one launch; the other
+ * elements are copied.  dtype BW_BF16 or BW_F32 for all four tensors (fp32
+ * arithmetic, one rounding).  Token (b, s) has the position positions[b][s] +
+ * pos_offset (positions int32 [B, S], NULL: s + pos_offset); a position outside
+ * [0, cache_seq_len) leaves the token as it is.  interleaved = 0: pairs
+ * (i, i + rotary_dim / 2), 1: pairs (2i, 2i + 1).  inverse = 1 applies the
+ * transpose, which is the gradient of the rotation: dQ from dQ_out.
+ * Q_out may be Q with the same strides (in place), otherwise the two must not
+ * overlap; the same for K.  Strides: elements of the (b, h, s) axes, NULL =
+ * contiguous, multiples of 16 bytes.  D: a multiple of 8, at most 512;
+ * rotary_dim: a multiple of 16. */
+BW_API int bw_rope(const void* Q, void* Q_out, const void* K, void* K_out, int dtype, int B, int Hq, int Hkv, int S,
+                   int D, const int64_t* q_strides, const int64_t* q_out_strides, const int64_t* k_strides,
+                   const int64_t* k_out_strides, const float* cos_sin_cache, int64_t cache_seq_len, int rotary_dim,
+                   const int* positions, int pos_offset, int interleaved, int inverse, void* stream);
+
+/* Writes T new tokens' K and V (bf16 [T, Hkv, D]; element strides of the
+ * (token, head) axes, NULL = contiguous, multiples of 8) into their slots of a
+ * paged cache [num_pages, page_size, Hkv, D] (slot = page * page_size + place):
+ * the caches of bw_gqa_decode_paged (cache_dtype BW_BF16) or of
+ * bw_gqa_decode_paged_fp8 (BW_E4M3).  With cos_sin_cache, K is rotated on the
+ * way as by bw_rope (positions int32 [T]); NULL leaves K as it is.
+ *   BW_E4M3: a row x[0..D) of one token and head is kept as e4m3 codes of
+ *   x / 2^e (round to nearest even) and the byte e + 127 in scales uint8
+ *   [num_pages, Hkv, 2, page_size] (0: K, 1: V); e is the smallest integer with
+ *   max|x| <= 448 * 2^e, clamped to [-100, 120], 0 for a row of zeros.  A
+ *   rotated row is quantised from fp32.  Infinities and NaN become NaN and do
+ *   not count towards the maximum.
+ * slots int64 [T]: a negative one skips its token (padding); one beyond the
+ * cache is skipped and reported as BW_ERR_INDEX by bw_stream_status.  The slots
+ * of a call must differ: a slot written twice in one call holds a mixture.
+ * page_size: 8, 16, 32, 64 or any multiple of 64.  T = 0 does nothing. */
+BW_API int bw_kv_cache_write(const void* K, const void* V, const int64_t* k_strides, const int64_t* v_strides, int T,
+                             int Hkv, int D, void* K_cache, void* V_cache, uint8_t* scales, int cache_dtype,
+                             int page_size, int num_pages, const int64_t* slots, const float* cos_sin_cache,
+                             int64_t cache_seq_len, int rotary_dim, const int* positions, int interleaved,
+                             void* stream);
+
+/* Reads spans of B sequences back from the paged cache as bf16 rows: tokens
+ * [kv_starts[b], kv_starts[b] + kv_lens[b]) (kv_starts NULL: from 0) go to the
+ * rows out_offsets[b] + 0, 1, ... of K_out and V_out [total_rows, Hkv, D], the
+ * layout of bw_gqa_decode and, through strides, of bw_gqa_causal_offset_fwd (a
+ * chunk's attention over its prefix).  Values are code * 2^e, exact in bf16
+ * (beyond its range: infinity).  Rows that no span covers are left as they
+ * are.  A span outside the block table or the output, and a token whose page is
+ * outside the cache, are skipped and reported as BW_ERR_INDEX. */
+BW_API int bw_kv_cache_read(const void* K_cache, const void* V_cache, const uint8_t* scales, int cache_dtype,
+                            int page_size, int num_pages, const int* block_table, int max_pages_per_seq,
+                            const int* kv_lens, const int* kv_starts, const int64_t* out_offsets, int B, int Hkv,
+                            int D, void* K_out, void* V_out, int64_t total_rows, void* stream);
+
+/* bw_gqa_decode_paged over the 8-bit cache of bw_kv_cache_write (K_cache,
+ * V_cache e4m3, scales): same meaning of every argument, without `chunk`: the
+ * tokens of all sequences are dealt evenly over the GPU, whatever their
+ * lengths, and the parts of a sequence are merged by a second kernel.  Keys and
+ * values enter at their exact values, Q is bf16, products and sums fp32; a
+ * token's weight is rounded to fp16 (relative 2^-11 of the largest weight * value
+ * scale).  O bf16, LSE natural log or NULL; a sequence without tokens gives
+ * O = 0 and LSE = -inf.  Codes, scales and table entries past kv_lens[b] are
+ * not used, whatever they hold.  A length beyond the table is cut to it.  A page
+ * outside the cache reads as page 0 and is reported as BW_ERR_INDEX.
+ * Workspace: bw_gqa_decode_paged_fp8_workspace_size(B, Hq, Hkv, D) bytes, 16-byte
+ * aligned, nothing in it needs a value before the call; calls that may overlap
+ * need one each. */
+BW_API size_t bw_gqa_decode_paged_fp8_workspace_size(int B, int Hq, int Hkv, int D);
+BW_API int bw_gqa_decode_paged_fp8(const void* Q, const void* K_cache, const void* V_cache, const uint8_t* scales,
+                                   const int* block_table, const int* kv_lens, void* O, float* LSE, int B, int Hq,
+                                   int Hkv, int D, int page_size, int num_pages, int max_pages_per_seq, float scale,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
 /* Host tensor layouts for bw_attn_fwd_host. */
 enum { BW_LAYOUT_BHSD = 0, BW_LAYOUT_BSHD = 1 };
 
@@ -235,7 +346,7 @@ BW_API int bw_attn_fwd_host(const void* Q, const void* K, const void* V, void* O
  * current device.  Every stream has its own word (the first 1023 distinct
  * streams of a device; later ones share one), so a call on one stream neither
  * sees nor clears the errors of calls on another.
- * Returns BW_OK, BW_ERR_TIMEOUT, BW_ERR_WORKSPACE or BW_ERR_CUDA. */
+ * Returns BW_OK, BW_ERR_TIMEOUT, BW_ERR_WORKSPACE, BW_ERR_INDEX or BW_ERR_CUDA. */
 BW_API int bw_stream_status(void* stream);
 
 /* Library options (process-wide).  Keys:
