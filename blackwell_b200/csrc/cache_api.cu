@@ -93,8 +93,7 @@ bool in_place(const bw::RopeTensor& t) {
   return t.in == t.out && t.in_sb == t.out_sb && t.in_sh == t.out_sh && t.in_ss == t.out_ss;
 }
 
-// Blocks of the decode: two dozen KB of shared memory a block would allow more
-// an SM; the token groups are at most this many blocks over the KV heads.
+// Most blocks of a decode (its workspace's size does not depend on the device).
 constexpr int kMaxDecodeBlocks = 1024;
 
 int decode_groups(int Hkv, int blocks) {
@@ -308,13 +307,20 @@ int bw_gqa_decode_paged_fp8(const void* Q, const void* K_cache, const void* V_ca
   p.max_pages = max_pages_per_seq;
   p.max_tokens = (int)max_tokens;
   p.scale_log2 = scale * 1.4426950408889634f;
-  p.groups = decode_groups(Hkv, sms * 4 < kMaxDecodeBlocks ? sms * 4 : kMaxDecodeBlocks);
+  const int blocks = bw::decode_fp8_blocks(sms, D, G);
+  p.groups = decode_groups(Hkv, blocks < kMaxDecodeBlocks ? blocks : kMaxDecodeBlocks);
+  bw::Fp8DecodeMaps maps;
+  const int64_t rows = (int64_t)num_pages * page_size;
+  const int box_rows = page_size < 64 ? page_size : 64;
+  if (bw::make_map_bytes(&maps.k, K_cache, (int64_t)Hkv * D, rows, D, box_rows) != BW_OK ||
+      bw::make_map_bytes(&maps.v, V_cache, (int64_t)Hkv * D, rows, D, box_rows) != BW_OK)
+    return BW_ERR_CUDA;
   const size_t parts = (size_t)(p.groups + B) * Hkv;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.prefix = reinterpret_cast<int*>(ws);
   p.lse_part = reinterpret_cast<float*>(ws + align256((size_t)(B + 1) * 4));
   p.o_part = reinterpret_cast<float*>(ws + align256((size_t)(B + 1) * 4) + align256(parts * G * 4));
-  return bw::launch_decode_fp8(p, static_cast<cudaStream_t>(stream)) == cudaSuccess ? BW_OK : BW_ERR_CUDA;
+  return bw::launch_decode_fp8(p, maps, static_cast<cudaStream_t>(stream)) == cudaSuccess ? BW_OK : BW_ERR_CUDA;
 }
 
 }  // extern "C"

@@ -23,7 +23,11 @@ namespace {
 
 constexpr int kTile = 64;      // tokens
 constexpr int kMinTiles = 4;   // tiles of a run, at least
-constexpr int kThreads = 128;
+constexpr int kWarps = 4;      // consumers
+constexpr int kThreads = 32 * (kWarps + 1);
+// Resident blocks an SM: registers (96 accumulators and Q fragments a thread in
+// the largest variant) and shared memory (about 67 KB a block).
+constexpr int blocks_per_sm(int D, int NT) { return D == 128 && NT == 2 ? 2 : 3; }
 
 // Tokens of sequence b: kv_lens[b], at least 0 and at most what its row of the
 // block table can hold.
@@ -61,109 +65,440 @@ __device__ __forceinline__ int tiles_per_group(int total, int groups) {
   return max((total + groups - 1) / groups, kMinTiles);
 }
 
+// ------------------------------------------------------------------ shared memory of a block
+// A stage is one tile: K and V codes of 64 tokens (pieces of bh = min(64, page
+// size) rows, D bytes a row, 16-byte chunks swizzled by the tensor map) and the
+// scale bytes [piece][K, V][bh].
 template <int D>
-__global__ void __launch_bounds__(kThreads) decode_fp8_kernel(const Fp8DecodeParams p) {
-  extern __shared__ int prefix[];
-  __shared__ int warp_sum[kThreads / 32];
-  __shared__ float qs[16][D], sc[16][kTile], vscale[kTile], m_s[16], l_s[16], corr_s[16];
-  tile_prefix(p, prefix, warp_sum);
-  const int tid = threadIdx.x;
+struct Cfg {
+  static constexpr int kHalf = kTile * D;            // K (or V) codes of a stage
+  static constexpr int kStage = 2 * kHalf;
+  static constexpr int kStages = D == 128 ? 4 : 8;   // 64 KB in flight a block
+  static constexpr int kScales = kStages * kStage;
+  static constexpr int kRed = kScales + kStages * 2 * kTile;    // m, l, M of 4 warps x 16 heads
+  static constexpr int kBars = kRed + 3 * kWarps * 16 * 4;
+  static constexpr int kPrefix = kBars + 256;
+};
+template <int D>
+struct Bars {
+  uint64_t full[Cfg<D>::kStages], empty[Cfg<D>::kStages];
+  int abort_flag;
+  int stop;   // what the consumers make of abort_flag at the end of a segment
+  int warp_sum[kThreads / 32];
+};
+static_assert(sizeof(Bars<64>) <= 256 && sizeof(Bars<128>) <= 256, "barriers fit their 256 bytes");
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
+// Untiled bulk copy of `bytes` (a multiple of 16, both addresses 16-byte aligned).
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+struct Segment {
+  int b, len, tok0, tok1;   // tokens [tok0, tok1) of sequence b
+};
+// The segment that begins at tile t0 of the run [t0, t1); t0 moves behind it.
+__device__ __forceinline__ Segment next_segment(const Fp8DecodeParams& p, const int* prefix, int& t0, int t1) {
+  int lo = 0, hi = p.B - 1;   // the last sequence that begins at or before t0, and so holds it
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (prefix[mid] <= t0) lo = mid; else hi = mid - 1;
+  }
+  Segment s;
+  s.b = lo;
+  s.len = seq_len(p, lo);
+  const int end = min(t1, prefix[lo + 1]);
+  s.tok0 = (t0 - prefix[lo]) * kTile;
+  s.tok1 = min((end - prefix[lo]) * kTile, s.len);
+  t0 = end;
+  return s;
+}
+
+// One producer warp streams the tiles of the block's run through a ring of
+// stages; four consumer warps take 16 tokens of a tile each, keep their own
+// running softmax and output, and merge at the end of a segment.
+//
+// The products run with tokens (then columns d) as the 16 rows of m16n8k16 and
+// the heads of the group as its 8 columns, so a group of up to 8 fills the
+// instruction (NT = 1; NT = 2 for up to 16):
+//   S^T[16 tokens, 8 heads] = K[16, D] Q^T,   O^T[D, 8] += V^T[D, 16] P^T[16, 8].
+// Codes go to f16 in registers (every e4m3 value is one): four bytes that
+// ldmatrix hands a lane are d = 4 q4 .. 4 q4 + 3 of its token, taken as the
+// k-columns 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9 of a step of 16 (Q in the same
+// order); of V they are columns 2g, 2g + 1 of two tokens, taken as the rows g
+// and g + 8 of a step of 16.
+//
+// Scales: x = (q k) 2^ek qs with the group's softmax scale and a power of two of
+// the Q row in qs (Q is brought to [1, 2) for f16).  2^ev must not be multiplied
+// into an f16 weight; the weight is 2^(x + ev - M) with M the running maximum of
+// x + ev, so the largest contribution is in [1, 2^8] whatever the scales are.
+// The denominator has its own reference m (the maximum of x): one more ex2 an
+// element.  Both references follow their maximum only when it has moved by more
+// than 2^8; m is per thread, M per warp (votes; shuffles only when it moves).
+template <int D, int NT>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
+    decode_fp8_kernel(const Fp8DecodeParams p, const __grid_constant__ Fp8DecodeMaps maps) {
+  using C = Cfg<D>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Bars<D>& bars = *reinterpret_cast<Bars<D>*>(smem + C::kBars);
+  int* prefix = reinterpret_cast<int*>(smem + C::kPrefix);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&bars.full[s], 1);
+      mbar_init(&bars.empty[s], kWarps);
+    }
+    bars.abort_flag = 0;
+    fence_mbar_init();
+  }
+  tile_prefix(p, prefix, bars.warp_sum);   // synchronises the block
+  asm volatile("griddepcontrol.launch_dependents;");
   const int grp = blockIdx.x / p.Hkv, kvh = blockIdx.x - grp * p.Hkv;
   const int total = prefix[p.B], per = tiles_per_group(total, p.groups);
   if (blockIdx.x == 0)
     for (int b = tid; b <= p.B; b += kThreads) p.prefix[b] = prefix[b];
   int t0 = min(grp * per, total);
   const int t1 = min(t0 + per, total);
+  const WaitCtl wc{&bars.abort_flag, p.err, p.timeout_ns, 48 + warp};
+  const uint32_t sbase = smem_u32(smem);
+  const int bh = p.page_size < kTile ? p.page_size : kTile;   // rows of a piece
+
+  if (warp == kWarps) {
+    // ------------------------------------------------------------ producer
+    // Lane = (piece of the tile, what of it): K codes, V codes, scale bytes (of K
+    // and V together in pages up to 64 tokens, else one lane each).
+    const int np = kTile / bh;
+    const int piece = lane % np, kind = lane / np;
+    const bool one_copy = p.page_size <= kTile;
+    const bool works = kind < (one_copy ? 3 : 4);
+    uint32_t n = 0;
+    bool ok = true;
+    while (ok && t0 < t1) {
+      const Segment sg = next_segment(p, prefix, t0, t1);
+      const int* bt = p.block_table + (int64_t)sg.b * p.max_pages;
+      const int last = ((sg.len - 1) / bh) * bh;   // pieces past the end read the last one again
+      auto row_of = [&](int t) -> int {            // first cache row of this lane's piece of the tile at t
+        const int tok = min(t + piece * bh, last);
+        const int pi = tok / p.page_size;
+        int page = bt[pi];
+        if ((unsigned)page >= (unsigned)p.num_pages) {
+          atomicCAS(p.err, 0, kErrIndexBit);
+          page = 0;
+        }
+        return page * p.page_size + (tok - pi * p.page_size);
+      };
+      int row = works ? row_of(sg.tok0) : 0;
+      for (int t = sg.tok0; t < sg.tok1; t += kTile, ++n) {
+        const uint32_t s = n % C::kStages;
+        bool got = true;
+        if (lane == 0) {
+          got = wc.wait(&bars.empty[s], ((n / C::kStages) & 1) ^ 1);
+          if (got) mbar_arrive_expect_tx(&bars.full[s], C::kStage + 2 * kTile);
+        }
+        if (!__shfl_sync(0xffffffffu, got, 0)) {
+          ok = false;
+          break;
+        }
+        if (works) {
+          uint8_t* dst = smem + s * C::kStage + piece * bh * D;
+          if (kind == 0) {
+            tma_load_2d(dst, &maps.k, &bars.full[s], kvh * D, row);
+          } else if (kind == 1) {
+            tma_load_2d(dst + C::kHalf, &maps.v, &bars.full[s], kvh * D, row);
+          } else {
+            const int page = row / p.page_size, place = row - page * p.page_size;
+            const uint8_t* src = p.scales + ((int64_t)page * p.Hkv + kvh) * 2 * p.page_size + place;
+            const uint32_t to = sbase + C::kScales + s * 2 * kTile;
+            if (one_copy) bulk_load(to + piece * 2 * bh, src, 2 * bh, &bars.full[s]);
+            else if (kind == 2) bulk_load(to, src, kTile, &bars.full[s]);
+            else bulk_load(to + kTile, src + p.page_size, kTile, &bars.full[s]);
+          }
+          if (t + kTile < sg.tok1) row = row_of(t + kTile);   // its page index arrives while the ring is full
+        }
+      }
+    }
+    __syncwarp();
+    if (!ok && lane == 0) {
+      for (uint32_t i = n > C::kStages ? n - C::kStages : 0; i < n; ++i)   // loads already in flight
+        drain_wait(&bars.full[i % C::kStages], (i / C::kStages) & 1, p.timeout_ns);
+    }
+    return;
+  }
+
+  // -------------------------------------------------------------- consumers
+  const int g = lane >> 2, q4 = lane & 3;
+  float* red_m = reinterpret_cast<float*>(smem + C::kRed);   // [warp][16]
+  float* red_l = red_m + kWarps * 16;
+  float* red_M = red_l + kWarps * 16;
+  // This lane's ldmatrix row: token (lane >> 3 & 1) * 8 + (lane & 7) of the warp's 16, chunk (lane >> 4) of a pair.
+  // 16-byte chunk c of tile row r lies at chunk c ^ (r & 7) of its row (128-byte rows), c ^ (r >> 1 & 3) (64-byte rows).
+  const int lrow = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+  const uint32_t row_off = (uint32_t)lrow * D;   // pieces follow one another: a row's place does not depend on bh
+  const uint32_t swz = D == 128 ? (lrow & 7) : ((lrow >> 1) & 3);
+  const uint32_t chunk0 = lane >> 4;
+  // scale bytes of tokens g and g + 8 of the warp's 16: K; V is bh further
+  uint32_t sc_off[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int tl = warp * 16 + g + 8 * i;
+    sc_off[i] = (uint32_t)(C::kScales + (tl / bh) * 2 * bh + tl % bh);
+  }
+  uint32_t n = 0;
   while (t0 < t1) {
-    int lo = 0, hi = p.B - 1;   // the last sequence that begins at or before t0 (and so holds it)
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (prefix[mid] <= t0) lo = mid; else hi = mid - 1;
-    }
-    const int b = lo, end = min(t1, prefix[b + 1]);
-    const int len = seq_len(p, b);
-    const int tok0 = (t0 - prefix[b]) * kTile, tok1 = min((end - prefix[b]) * kTile, len);
-    for (int i = tid; i < p.G * D; i += kThreads)
-      qs[i / D][i % D] = __bfloat162float(static_cast<const __nv_bfloat16*>(p.Q)[((int64_t)b * p.Hq + kvh * p.G) * D + i]);
-    if (tid < 16) {
-      m_s[tid] = -INFINITY;
-      l_s[tid] = 0.f;
-    }
-    float acc[16 * D / kThreads] = {};
-    __syncthreads();
-    for (int t = tok0; t < tok1; t += kTile) {
-      const int nt = min(kTile, tok1 - t);
-      for (int i = tid; i < p.G * kTile; i += kThreads) {
-        const int g = i / kTile, j = i % kTile;
-        float s = -INFINITY;
-        if (j < nt) {
-          const int at = t + j, pi = at / p.page_size, place = at - pi * p.page_size;
-          int page = p.block_table[(int64_t)b * p.max_pages + pi];
-          if (page < 0 || page >= p.num_pages) {
-            atomicCAS(p.err, 0, kErrIndexBit);
-            page = 0;
-          }
-          const uint8_t* k = static_cast<const uint8_t*>(p.k_cache) + (((int64_t)page * p.page_size + place) * p.Hkv + kvh) * D;
-          const uint8_t* bytes = p.scales + (((int64_t)page * p.Hkv + kvh) * 2) * p.page_size + place;
-          float dot = 0.f;
-          for (int d = 0; d < D; d += 2) {
-            const float2 kk = e4m3x2_to_f32(*reinterpret_cast<const uint16_t*>(k + d));
-            dot = fmaf(qs[g][d], kk.x, fmaf(qs[g][d + 1], kk.y, dot));
-          }
-          s = dot * __uint_as_float((uint32_t)bytes[0] << 23) * p.scale_log2;
-          if (g == 0) vscale[j] = __uint_as_float((uint32_t)bytes[p.page_size] << 23);
-        }
-        sc[g][j] = s;
-      }
-      __syncthreads();
-      if (tid < p.G) {
-        float m = m_s[tid];
-        for (int j = 0; j < nt; ++j) m = fmaxf(m, sc[tid][j]);
-        const float sub = m == -INFINITY ? 0.f : m;
-        corr_s[tid] = exp2f(m_s[tid] - sub);
-        float l = l_s[tid] * corr_s[tid];
-        for (int j = 0; j < nt; ++j) {
-          sc[tid][j] = exp2f(sc[tid][j] - sub);
-          l += sc[tid][j];
-        }
-        m_s[tid] = m;
-        l_s[tid] = l;
-      }
-      __syncthreads();
-      for (int j = 0; j < nt; ++j) {
-        const int at = t + j, pi = at / p.page_size, place = at - pi * p.page_size;
-        int page = p.block_table[(int64_t)b * p.max_pages + pi];
-        if (page < 0 || page >= p.num_pages) page = 0;
-        const uint8_t* v = static_cast<const uint8_t*>(p.v_cache) + (((int64_t)page * p.page_size + place) * p.Hkv + kvh) * D;
+    const Segment sg = next_segment(p, prefix, t0, t1);
+    // Q of head (n tile) + g as f16, brought to [1, 2) by a power of two; columns in the codes' order
+    uint32_t qb[NT][D / 16][2];
+    float qs[NT][2];
 #pragma unroll
-        for (int u = 0; u < 16 * D / kThreads; ++u) {
-          const int i = tid + u * kThreads, g = i / D, d = i % D;
-          if (g < p.G) {
-            if (j == 0) acc[u] *= corr_s[g];
-            acc[u] = fmaf(sc[g][j] * vscale[j], e4m3x2_to_f32(v[d]).x, acc[u]);
+    for (int nt = 0; nt < NT; ++nt) {
+      const int h = nt * 8 + g;
+      const __nv_bfloat16* Q = static_cast<const __nv_bfloat16*>(p.Q) + ((int64_t)sg.b * p.Hq + kvh * p.G + h) * D;
+      uint2 raw[D / 16];
+      uint32_t top = 0;   // largest magnitude's bits
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        raw[j] = h < p.G ? *reinterpret_cast<const uint2*>(Q + 16 * j + 4 * q4) : make_uint2(0u, 0u);
+        top = max(top, max(max(raw[j].x & 0x7fffu, (raw[j].x >> 16) & 0x7fffu),
+                           max(raw[j].y & 0x7fffu, (raw[j].y >> 16) & 0x7fffu)));
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int ex = min(max((int)(top >> 7), 2), 252);   // biased exponent
+      const float down = __uint_as_float((uint32_t)(254 - ex) << 23), up = __uint_as_float((uint32_t)ex << 23);
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        qb[nt][j][0] = f16x2(__uint_as_float(raw[j].x << 16) * down, __uint_as_float(raw[j].x & 0xffff0000u) * down);
+        qb[nt][j][1] = f16x2(__uint_as_float(raw[j].y << 16) * down, __uint_as_float(raw[j].y & 0xffff0000u) * down);
+      }
+      const float mine = p.scale_log2 * up;
+      qs[nt][0] = __shfl_sync(0xffffffffu, mine, 8 * q4);       // of head 2 q4 (held by lanes 4 * head ..)
+      qs[nt][1] = __shfl_sync(0xffffffffu, mine, 8 * q4 + 4);
+    }
+    float o[NT][D / 16][4];
+    float m[NT][2], l[NT][2], M[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) o[nt][c][0] = o[nt][c][1] = o[nt][c][2] = o[nt][c][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        m[nt][j] = M[nt][j] = -INFINITY;
+        l[nt][j] = 0.f;
+      }
+    }
+    uint32_t s = 0;
+    for (int t = sg.tok0; t < sg.tok1; t += kTile, ++n) {
+      s = n % C::kStages;
+      // On a timeout the warp still goes through the merge below, so that the
+      // barriers stay matched.
+      if (!wc.wait(&bars.full[s], (n / C::kStages) & 1)) break;
+      const int left = sg.tok1 - (t + warp * 16);   // tokens of this warp that exist
+      if (left > 0) {
+        const uint32_t kb = sbase + s * C::kStage + row_off, vb = kb + C::kHalf;
+        // S^T: two chains of products
+        float acc[NT][2][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
+#pragma unroll
+        for (int j = 0; j < D / 16; j += 2) {
+          uint32_t r[4];
+          ldsm_x4(kb + (((j + chunk0) ^ swz) << 4), r);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t a0 = e4m3x2_to_f16x2(r[2 * i]), a2 = e4m3x2_to_f16x2(r[2 * i] >> 16);
+            const uint32_t a1 = e4m3x2_to_f16x2(r[2 * i + 1]), a3 = e4m3x2_to_f16x2(r[2 * i + 1] >> 16);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt][i], a0, a1, a2, a3, qb[nt][j + i][0], qb[nt][j + i][1]);
+          }
+        }
+        const uint8_t* sc = smem + s * 2 * kTile;
+        const uint32_t kb0 = sc[sc_off[0]], kb1 = sc[sc_off[1]], vb0 = sc[sc_off[0] + bh], vb1 = sc[sc_off[1] + bh];
+        const float ks0 = __uint_as_float(kb0 << 23), ks1 = __uint_as_float(kb1 << 23);
+        const float ev0 = (float)((int)vb0 - 127), ev1 = (float)((int)vb1 - 127);
+        const bool in0 = g < left, in1 = g + 8 < left;
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float x[2][2], y[2][2];   // [head 2 q4 + j][token g + 8 i]
+          bool moved = false;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            x[j][0] = in0 ? (acc[nt][0][j] + acc[nt][1][j]) * ks0 * qs[nt][j] : -INFINITY;
+            x[j][1] = in1 ? (acc[nt][0][2 + j] + acc[nt][1][2 + j]) * ks1 * qs[nt][j] : -INFINITY;
+            const float mx = fmaxf(x[j][0], x[j][1]);
+            if (mx > m[nt][j] + 8.f) {
+              l[nt][j] *= ex2f(m[nt][j] - mx);
+              m[nt][j] = mx;
+            }
+            const float sub = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
+            l[nt][j] += ex2f(x[j][0] - sub) + ex2f(x[j][1] - sub);
+            y[j][0] = in0 ? x[j][0] + ev0 : -INFINITY;
+            y[j][1] = in1 ? x[j][1] + ev1 : -INFINITY;
+            moved |= fmaxf(y[j][0], y[j][1]) > M[nt][j] + 8.f;
+          }
+          if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float mx = fmaxf(y[j][0], y[j][1]);
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              mx = fmaxf(mx, M[nt][j]);
+              const float corr = mx == -INFINITY ? 1.f : ex2f(M[nt][j] - mx);
+              M[nt][j] = mx;
+#pragma unroll
+              for (int c = 0; c < D / 16; ++c) {
+                o[nt][c][j] *= corr;
+                o[nt][c][2 + j] *= corr;
+              }
+            }
+          }
+          const float M0 = M[nt][0] == -INFINITY ? 0.f : M[nt][0], M1 = M[nt][1] == -INFINITY ? 0.f : M[nt][1];
+          pb[nt][0] = transpose8x8(f16x2(ex2f(y[0][0] - M0), ex2f(y[1][0] - M1)));
+          pb[nt][1] = transpose8x8(f16x2(ex2f(y[0][1] - M0), ex2f(y[1][1] - M1)));
+        }
+        // O^T: bytes (t0 2g, t0 2g+1, t1 2g, t1 2g+1) -> (t0, t1) of 2g and of 2g + 1; a token past the end is
+        // picked as zero, whatever its codes are (a weight of 0 would not silence a NaN)
+        const uint32_t sel0 = (2 * q4 < left ? 0x0100u : 0x0404u) | (2 * q4 + 1 < left ? 0x3020u : 0x4040u);
+        const uint32_t sel1 = (2 * q4 + 8 < left ? 0x0100u : 0x0404u) | (2 * q4 + 9 < left ? 0x3020u : 0x4040u);
+#pragma unroll
+        for (int c = 0; c < D / 16; c += 2) {
+          uint32_t r[4];
+          ldsm_x4_t(vb + (((c + chunk0) ^ swz) << 4), r);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t w0 = __byte_perm(r[2 * i], 0, sel0), w1 = __byte_perm(r[2 * i + 1], 0, sel1);
+            const uint32_t a0 = e4m3x2_to_f16x2(w0), a1 = e4m3x2_to_f16x2(w0 >> 16);
+            const uint32_t a2 = e4m3x2_to_f16x2(w1), a3 = e4m3x2_to_f16x2(w1 >> 16);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][c + i], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
           }
         }
       }
-      __syncthreads();
-    }
-    const bool whole = tok0 == 0 && tok1 == len;
-    const int64_t part = (int64_t)(grp + b) * p.Hkv + kvh;
-#pragma unroll
-    for (int u = 0; u < 16 * D / kThreads; ++u) {
-      const int i = tid + u * kThreads, g = i / D, d = i % D;
-      if (g >= p.G) continue;
-      const float o = acc[u] / l_s[g];
-      const int64_t row = (int64_t)b * p.Hq + kvh * p.G + g;
-      if (whole) static_cast<__nv_bfloat16*>(p.O)[row * D + d] = __float2bfloat16(o);
-      else p.o_part[(part * p.G + g) * D + d] = o;
-      if (d == 0) {
-        const float lse = (m_s[g] + log2f(l_s[g])) * 0.69314718055994531f;
-        if (!whole) p.lse_part[part * p.G + g] = lse;
-        else if (p.LSE) p.LSE[row] = lse;
+      // the last stage of a segment is kept for the merge
+      if (t + kTile < sg.tok1) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.empty[s]);
       }
     }
-    __syncthreads();
-    t0 = end;
+
+    // ---- merge the four warps: references and sums of every head, then the
+    // outputs through the last stage (4 warps x 8 heads x D floats = its codes)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float mm = m[nt][j];
+        mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, 4));
+        mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, 8));
+        mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, 16));
+        float ll = l[nt][j] * (m[nt][j] == -INFINITY ? 1.f : ex2f(m[nt][j] - mm));
+        ll += __shfl_xor_sync(0xffffffffu, ll, 4);
+        ll += __shfl_xor_sync(0xffffffffu, ll, 8);
+        ll += __shfl_xor_sync(0xffffffffu, ll, 16);
+        if (g == 0) {
+          const int h = warp * 16 + nt * 8 + 2 * q4 + j;
+          red_m[h] = mm;
+          red_l[h] = ll;
+          red_M[h] = M[nt][j];
+        }
+      }
+    const bool whole = sg.tok0 == 0 && sg.tok1 == sg.len;
+    const int64_t part = (int64_t)(grp + sg.b) * p.Hkv + kvh;
+    float* part_o = reinterpret_cast<float*>(smem + s * C::kStage);   // [warp][8][D]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      consumer_sync();   // the stage's codes (or the previous heads' outputs) have been read
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          *reinterpret_cast<float2*>(part_o + (warp * 8 + 2 * q4 + j) * D + 16 * c + 2 * g) =
+              make_float2(o[nt][c][j], o[nt][c][2 + j]);
+      consumer_sync();
+      for (int i = tid; i < 8 * D / 4; i += kWarps * 32) {
+        const int hl = i / (D / 4), d = (i - hl * (D / 4)) * 4, h = nt * 8 + hl;
+        if (h >= p.G) break;
+        float mx = -INFINITY, Mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          mx = fmaxf(mx, red_m[w * 16 + h]);
+          Mx = fmaxf(Mx, red_M[w * 16 + h]);
+        }
+        float sum = 0.f;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float mw = red_m[w * 16 + h], Mw = red_M[w * 16 + h];
+          sum += red_l[w * 16 + h] * (mw == -INFINITY ? 1.f : ex2f(mw - mx));
+          const float f = Mw == -INFINITY ? 1.f : ex2f(Mw - Mx);
+          const float4 v = *reinterpret_cast<const float4*>(part_o + (w * 8 + hl) * D + d);
+          a.x = fmaf(f, v.x, a.x);
+          a.y = fmaf(f, v.y, a.y);
+          a.z = fmaf(f, v.z, a.z);
+          a.w = fmaf(f, v.w, a.w);
+        }
+        // o = a 2^Mx / (sum 2^mx); both powers may be far out, their quotient is the values' scale
+        const float f = (Mx == -INFINITY ? 1.f : ex2f(Mx - mx)) / sum;
+        a.x *= f; a.y *= f; a.z *= f; a.w *= f;
+        const int64_t row = (int64_t)sg.b * p.Hq + kvh * p.G + h;
+        if (whole)
+          *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.O) + row * D + d) =
+              make_uint2(f32_to_bf16x2(a.x, a.y), f32_to_bf16x2(a.z, a.w));
+        else
+          *reinterpret_cast<float4*>(p.o_part + (part * p.G + h) * D + d) = a;
+        if (d == 0) {
+          const float lse = (mx + __log2f(sum)) * 0.69314718055994531f;
+          if (!whole) p.lse_part[part * p.G + h] = lse;
+          else if (p.LSE) p.LSE[row] = lse;
+        }
+      }
+    }
+    // After a wait that ran out all four warps stop at the same segment, so that
+    // none waits at a barrier for one that has left.
+    if (tid == 0) bars.stop = *wc.abort_flag;
+    fence_proxy_async_smem();   // the stage goes back to the copies
+    consumer_sync();
+    if (lane == 0) mbar_arrive(&bars.empty[s]);
+    if (*(volatile int*)&bars.stop) break;
   }
 }
 
@@ -175,6 +510,7 @@ __global__ void __launch_bounds__(128) decode_fp8_join_kernel(const Fp8DecodePar
   constexpr int kRows = 128 / kLanes;        // segments in flight
   __shared__ float4 part[kRows][kLanes];
   __shared__ float wsum_s[kRows], max_s[4];
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // the segments are written
   const int hq = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int kvh = hq / p.G, g = hq - kvh * p.G;
   const int first = p.prefix[b], last = p.prefix[b + 1], per = tiles_per_group(p.prefix[p.B], p.groups);
@@ -224,20 +560,36 @@ __global__ void __launch_bounds__(128) decode_fp8_join_kernel(const Fp8DecodePar
   }
 }
 
-template <int D>
-cudaError_t launch(const Fp8DecodeParams& p, cudaStream_t stream) {
-  const int bytes = (p.B + 1) * 4;
-  decode_fp8_kernel<D><<<p.groups * p.Hkv, kThreads, bytes, stream>>>(p);
-  cudaError_t e = cudaGetLastError();
+template <int D, int NT>
+cudaError_t launch(const Fp8DecodeParams& p, const Fp8DecodeMaps& maps, cudaStream_t stream) {
+  auto kern = decode_fp8_kernel<D, NT>;
+  const int bytes = Cfg<D>::kPrefix + (p.B + 1) * 4 + 1024;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
-  decode_fp8_join_kernel<D><<<dim3(p.Hq, p.B), 128, 0, stream>>>(p);
-  return cudaGetLastError();
+  kern<<<p.groups * p.Hkv, kThreads, bytes, stream>>>(p, maps);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  // The join's blocks start while the decode's last ones finish and wait there
+  // for its results (griddepcontrol), which takes the launch out of the path.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(p.Hq, p.B);
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, decode_fp8_join_kernel<D>, p);
 }
 
 }  // namespace
 
-cudaError_t launch_decode_fp8(const Fp8DecodeParams& p, cudaStream_t stream) {
-  return p.D == 128 ? launch<128>(p, stream) : launch<64>(p, stream);
+int decode_fp8_blocks(int num_sms, int D, int G) { return num_sms * blocks_per_sm(D, G <= 8 ? 1 : 2); }
+
+cudaError_t launch_decode_fp8(const Fp8DecodeParams& p, const Fp8DecodeMaps& maps, cudaStream_t stream) {
+  if (p.D == 128) return p.G <= 8 ? launch<128, 1>(p, maps, stream) : launch<128, 2>(p, maps, stream);
+  return p.G <= 8 ? launch<64, 1>(p, maps, stream) : launch<64, 2>(p, maps, stream);
 }
 
 }  // namespace bw

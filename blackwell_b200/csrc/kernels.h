@@ -224,7 +224,17 @@ struct Fp8DecodeParams {
   int* err;
   uint64_t timeout_ns;
 };
-cudaError_t launch_decode_fp8(const Fp8DecodeParams& p, cudaStream_t stream);
+struct Fp8DecodeMaps {
+  // 2-D (Hkv * D, rows) bytes over K or V codes; box (D, min(64, page_size)),
+  // swizzled over its row of D = 128 or 64 bytes
+  CUtensorMap k, v;
+};
+// Blocks of the decode on a device of num_sms SMs (a full wave).
+int decode_fp8_blocks(int num_sms, int D, int G);
+cudaError_t launch_decode_fp8(const Fp8DecodeParams& p, const Fp8DecodeMaps& maps, cudaStream_t stream);
+
+// 2-D byte map with a box of (128 or 64 swizzled bytes, rows) (api.cu).
+int make_map_bytes(CUtensorMap* m, const void* base, int64_t row_bytes, int64_t rows, int box_bytes, int box_rows);
 
 // What an entry point outside api.cu needs of the current device: SM count, the
 // error word of `stream`, the bound on device-side waits.  Returns a status code.
