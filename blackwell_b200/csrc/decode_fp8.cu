@@ -343,8 +343,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
           ldsm_x4(kb + (((j + chunk0) ^ swz) << 4), r);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const uint32_t a0 = e4m3x2_to_f16x2(r[2 * i]), a2 = e4m3x2_to_f16x2(r[2 * i] >> 16);
-            const uint32_t a1 = e4m3x2_to_f16x2(r[2 * i + 1]), a3 = e4m3x2_to_f16x2(r[2 * i + 1] >> 16);
+            uint32_t a0, a1, a2, a3;
+            e4m3x4_to_f16x4(r[2 * i], a0, a2);
+            e4m3x4_to_f16x4(r[2 * i + 1], a1, a3);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt][i], a0, a1, a2, a3, qb[nt][j + i][0], qb[nt][j + i][1]);
           }
@@ -405,9 +406,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
           ldsm_x4_t(vb + (((c + chunk0) ^ swz) << 4), r);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const uint32_t w0 = __byte_perm(r[2 * i], 0, sel0), w1 = __byte_perm(r[2 * i + 1], 0, sel1);
-            const uint32_t a0 = e4m3x2_to_f16x2(w0), a1 = e4m3x2_to_f16x2(w0 >> 16);
-            const uint32_t a2 = e4m3x2_to_f16x2(w1), a3 = e4m3x2_to_f16x2(w1 >> 16);
+            uint32_t a0, a1, a2, a3;
+            e4m3x4_to_f16x4(__byte_perm(r[2 * i], 0, sel0), a0, a1);
+            e4m3x4_to_f16x4(__byte_perm(r[2 * i + 1], 0, sel1), a2, a3);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][c + i], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
           }

@@ -150,9 +150,10 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvReadParams p)
         uint32_t o[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 a = e4m3x2_to_f32(cw[j]), d = e4m3x2_to_f32(cw[j] >> 16);
-          o[2 * j] = f32_to_bf16x2(a.x * sc, a.y * sc);
-          o[2 * j + 1] = f32_to_bf16x2(d.x * sc, d.y * sc);
+          float f[4];
+          e4m3x4_to_f32(cw[j], f);
+          o[2 * j] = f32_to_bf16x2(f[0] * sc, f[1] * sc);
+          o[2 * j + 1] = f32_to_bf16x2(f[2] * sc, f[3] * sc);
         }
         out[0] = make_uint4(o[0], o[1], o[2], o[3]);
         out[1] = make_uint4(o[4], o[5], o[6], o[7]);

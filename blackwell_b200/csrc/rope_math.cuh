@@ -63,14 +63,22 @@ __device__ __forceinline__ uint32_t f32_to_e4m3x4(float a, float b, float c, flo
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
   return lo | (hi << 16);
 }
-// Two codes (low 16 bits) -> half2 bits; every e4m3 value is an f16 value.
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xffffu), __NV_E4M3);
-  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+// Four codes -> two half2 (lo: bytes 0 and 1, hi: bytes 2 and 3); every e4m3 value is
+// an f16 value.
+__device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\t"
+      "mov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(four));
 }
-__device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t two) {
-  const uint32_t h = e4m3x2_to_f16x2(two);
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+__device__ __forceinline__ void e4m3x4_to_f32(uint32_t four, float* x) {
+  uint32_t lo, hi;
+  e4m3x4_to_f16x4(four, lo, hi);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
 }
 
 }  // namespace bw
