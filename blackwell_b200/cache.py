@@ -23,15 +23,27 @@ _SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
 _E4M3 = torch.float8_e4m3fn
 
 
-def _on_gpu(**tensors):
-    """Every tensor given lies on the current CUDA device."""
-    for name, t in tensors.items():
-        if t is not None and not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor")
-    dev = torch.cuda.current_device()
-    for name, t in tensors.items():
-        if t is not None and t.device.index != dev:
-            raise ValueError(f"{name} is on {t.device}, the current device is cuda:{dev}")
+_A3, _A2 = ctypes.c_int64 * 3, ctypes.c_int64 * 2
+# The current stream's handle without a Stream object around it (3 us of a call's 17 otherwise).
+_raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch.cuda.current_device
+
+
+def _on_gpu(*tensors):
+    """The index of the current CUDA device, on which every tensor given lies."""
+    first = None
+    for t in tensors:
+        if t is not None:
+            d = t.get_device()
+            if d < 0:
+                raise ValueError(f"expected CUDA tensors, got a {t.dtype} {tuple(t.shape)} tensor on {t.device}")
+            if d != first:
+                if first is not None:
+                    raise ValueError(f"the tensors are on different devices (cuda:{first} and cuda:{d})")
+                first = d
+    dev = _device()
+    if first is not None and first != dev:
+        raise ValueError(f"the tensors are on cuda:{first}, the current device is cuda:{dev}")
+    return dev
 
 
 def _want(name, t, dtype, shape):
@@ -47,10 +59,6 @@ def _table(t):
         raise ValueError("cos_sin_cache must be a contiguous fp32 [length, rotary_dim] tensor")
 
 
-def _stream():
-    return torch.cuda.current_stream().cuda_stream
-
-
 def rope_table(length, rotary_dim, base=10000.0, scaling="none", factor=1.0, original_length=0, attention_factor=0.0,
                beta_fast=0.0, beta_slow=0.0, low_freq_factor=0.0, high_freq_factor=0.0, first=0, out=None):
     """cos | sin table fp32 [length, rotary_dim] of the positions first .. first + length - 1.
@@ -62,26 +70,27 @@ def rope_table(length, rotary_dim, base=10000.0, scaling="none", factor=1.0, ori
     if scaling not in _SCALINGS:
         raise ValueError(f"scaling must be one of {sorted(_SCALINGS)}, got {scaling!r}")
     length, rotary_dim = int(length), int(rotary_dim)
-    if out is not None:
-        _on_gpu(out=out)
+    dev = _on_gpu(out)
+    if out is None:
+        out = torch.empty((length, rotary_dim), dtype=torch.float32, device=torch.device("cuda", dev))
+    else:
         _want("out", out, torch.float32, (length, rotary_dim))
-    elif length > 0 and rotary_dim > 0:
-        out = torch.empty((length, rotary_dim), dtype=torch.float32,
-                          device=torch.device("cuda", torch.cuda.current_device()))
     s = _ffi.BwRopeScaling(_SCALINGS[scaling], base, factor, original_length, attention_factor, beta_fast, beta_slow,
                            low_freq_factor, high_freq_factor)
-    rc = _ffi.lib().bw_rope_table(out.data_ptr() if out is not None else 1 << 20, length, rotary_dim, int(first),
-                                  ctypes.addressof(s), _stream())
+    rc = _ffi.lib().bw_rope_table(out.data_ptr(), length, rotary_dim, int(first), ctypes.addressof(s),
+                                  _raw_stream(dev))
     _ffi.check(rc, "bw_rope_table")
     return out
 
 
-def _bhs(name, t, D):
-    """Strides of a [B, H, S, D] tensor, or of a [tokens, H, D] one seen as [1, H, tokens, D]."""
+def _bhs(name, t):
+    """Strides of a [B, H, S, D] tensor or of [tokens, H, D] (B = tokens, S = 1); None: contiguous."""
+    if t.is_contiguous():
+        return None
     st = t.stride()
-    if st[-1] != 1 and D > 1:
+    if st[-1] != 1:
         raise ValueError(f"{name} must have a contiguous last dimension")
-    return (ctypes.c_int64 * 3)(*(st[:3] if len(st) == 4 else (0, st[1], st[0])))
+    return _A3(st[0], st[1], st[2] if len(st) == 4 else 0)
 
 
 def rope(q, k, cos_sin_cache, positions=None, pos_offset=0, interleaved=False, inverse=False, q_out=None, k_out=None):
@@ -94,46 +103,51 @@ def rope(q, k, cos_sin_cache, positions=None, pos_offset=0, interleaved=False, i
     is copied.  interleaved: pairs (2i, 2i + 1) instead of (i, i + R / 2).
     inverse: the transposed rotation, which maps gradients of the outputs to
     gradients of the inputs.  q_out may be q (in place)."""
-    nd = q.dim()
-    if nd not in (3, 4):
-        raise ValueError("q must be [B, H, S, D] or [tokens, H, D]")
-    if q.dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"q must be bfloat16 or float32, got {q.dtype}")
-    _table(cos_sin_cache)
+    nd, dtype, shape = q.dim(), q.dtype, q.shape
     if nd == 4:
-        B, Hq, S, D = q.shape
-        Hkv = k.shape[1] if k is not None else 0
-        k_shape, pos_shape = (B, Hkv, S, D), (B, S)
+        B, Hq, S, D = shape
+    elif nd == 3:
+        (B, Hq, D), S = shape, 1
     else:
-        (S, Hq, D), B = q.shape, 1
-        Hkv = k.shape[1] if k is not None else 0
-        k_shape, pos_shape = (S, Hkv, D), (S,)
-    if k is not None and (k.shape != k_shape or k.dtype != q.dtype):
-        raise ValueError(f"k must be a {q.dtype} {k_shape} tensor, got {k.dtype} {tuple(k.shape)}")
+        raise ValueError("q must be [B, H, S, D] or [tokens, H, D]")
+    if dtype != torch.bfloat16 and dtype != torch.float32:
+        raise TypeError(f"q must be bfloat16 or float32, got {dtype}")
+    _table(cos_sin_cache)
     if q_out is None:
         q_out = torch.empty_like(q)
+    elif q_out.shape != shape or q_out.dtype != dtype:
+        raise ValueError(f"q_out must be a {dtype} {tuple(shape)} tensor")
     if k is None:
         if k_out is not None:
             raise ValueError("k_out without k")
-    elif k_out is None:
-        k_out = torch.empty_like(k)
-    for name, t, ref in (("q_out", q_out, q), ("k_out", k_out, k)):
-        if t is not None and (t.shape != ref.shape or t.dtype != ref.dtype):
-            raise ValueError(f"{name} must be a {ref.dtype} {tuple(ref.shape)} tensor")
-    _on_gpu(q=q, k=k, cos_sin_cache=cos_sin_cache, positions=positions, q_out=q_out, k_out=k_out)
+        Hkv, kp, kop, ks, kos = 0, None, None, None, None
+    else:
+        k_shape = k.shape
+        if k.dim() != nd or k.dtype != dtype or k_shape[0] != B or k_shape[2:] != shape[2:]:
+            raise ValueError(f"k must be q's {dtype} tensor but for the number of heads, got {k.dtype} {tuple(k_shape)}")
+        Hkv = k_shape[1]
+        if k_out is None:
+            k_out = torch.empty_like(k)
+        elif k_out.shape != k_shape or k_out.dtype != dtype:
+            raise ValueError(f"k_out must be a {dtype} {tuple(k_shape)} tensor")
+        kp, kop, ks, kos = k.data_ptr(), k_out.data_ptr(), _bhs("k", k), _bhs("k_out", k_out)
+    dev = _on_gpu(q, k, cos_sin_cache, positions, q_out, k_out)
+    pos = None
     if positions is not None:
-        _want("positions", positions, torch.int32, pos_shape)
+        _want("positions", positions, torch.int32, (B, S) if nd == 4 else (B,))
+        pos = positions.data_ptr()
+    elif nd == 3:   # 0, 1, ... along the tokens: one sequence
+        B, S = 1, B
+        turn = lambda t, st: None if t is None else _A3(0, t.stride(1), t.stride(0))  # noqa: E731
     if q.numel() == 0:
         return q_out, k_out
-    ks = kos = None
-    if k is not None:
-        ks, kos = _bhs("k", k, D), _bhs("k_out", k_out, D)
+    qs, qos = _bhs("q", q), _bhs("q_out", q_out)
+    if pos is None and nd == 3:
+        qs, qos, ks, kos = turn(q, qs), turn(q_out, qos), turn(k, ks), turn(k_out, kos)
     rc = _ffi.lib().bw_rope(
-        q.data_ptr(), q_out.data_ptr(), k.data_ptr() if k is not None else None,
-        k_out.data_ptr() if k is not None else None, _ffi.BW_BF16 if q.dtype == torch.bfloat16 else _ffi.BW_F32,
-        B, Hq, Hkv, S, D, _bhs("q", q, D), _bhs("q_out", q_out, D), ks, kos, cos_sin_cache.data_ptr(),
-        cos_sin_cache.shape[0], cos_sin_cache.shape[1], positions.data_ptr() if positions is not None else None,
-        int(pos_offset), int(bool(interleaved)), int(bool(inverse)), _stream())
+        q.data_ptr(), q_out.data_ptr(), kp, kop, _ffi.BW_BF16 if dtype == torch.bfloat16 else _ffi.BW_F32, B, Hq, Hkv,
+        S, D, qs, qos, ks, kos, cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], cos_sin_cache.shape[1], pos,
+        int(pos_offset), int(bool(interleaved)), int(bool(inverse)), _raw_stream(dev))
     _ffi.check(rc, "bw_rope")
     return q_out, k_out
 
@@ -185,12 +199,11 @@ def kv_cache_write(k, v, k_cache, v_cache, slots, scales=None, cos_sin_cache=Non
         length, R = cos_sin_cache.shape
     elif positions is not None:
         raise ValueError("positions need cos_sin_cache")
-    _on_gpu(k=k, v=v, k_cache=k_cache, v_cache=v_cache, slots=slots, scales=scales, cos_sin_cache=cos_sin_cache,
-            positions=positions)
+    dev = _on_gpu(k, v, k_cache, v_cache, slots, scales, cos_sin_cache, positions)
     rc = _ffi.lib().bw_kv_cache_write(
-        k.data_ptr(), v.data_ptr(), (ctypes.c_int64 * 2)(ks[0], ks[1]), (ctypes.c_int64 * 2)(vs[0], vs[1]), T, Hkv, D,
-        k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr() if scales is not None else None, code, page_size,
-        num_pages, slots.data_ptr(), table, length, R, pos, int(bool(interleaved)), _stream())
+        k.data_ptr(), v.data_ptr(), _A2(ks[0], ks[1]), _A2(vs[0], vs[1]), T, Hkv, D, k_cache.data_ptr(),
+        v_cache.data_ptr(), scales.data_ptr() if scales is not None else None, code, page_size, num_pages,
+        slots.data_ptr(), table, length, R, pos, int(bool(interleaved)), _raw_stream(dev))
     _ffi.check(rc, "bw_kv_cache_write")
     return k_cache, v_cache
 
@@ -216,8 +229,7 @@ def kv_cache_read(k_cache, v_cache, block_table, kv_lens, out_offsets, scales=No
         if k_out is None:
             raise ValueError("give k_out and v_out, or total_rows")
         total_rows = k_out.shape[0]
-    _on_gpu(k_cache=k_cache, v_cache=v_cache, block_table=block_table, kv_lens=kv_lens, out_offsets=out_offsets,
-            scales=scales, kv_starts=kv_starts, k_out=k_out, v_out=v_out)
+    dev = _on_gpu(k_cache, v_cache, block_table, kv_lens, out_offsets, scales, kv_starts, k_out, v_out)
     shape = (int(total_rows), Hkv, D)
     if k_out is None:
         k_out = torch.empty(shape, dtype=torch.bfloat16, device=k_cache.device)
@@ -229,7 +241,7 @@ def kv_cache_read(k_cache, v_cache, block_table, kv_lens, out_offsets, scales=No
         k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr() if scales is not None else None, code, page_size,
         num_pages, block_table.data_ptr(), block_table.shape[1], kv_lens.data_ptr(),
         kv_starts.data_ptr() if kv_starts is not None else None, out_offsets.data_ptr(), B, Hkv, D, k_out.data_ptr(),
-        v_out.data_ptr(), shape[0], _stream())
+        v_out.data_ptr(), shape[0], _raw_stream(dev))
     _ffi.check(rc, "bw_kv_cache_read")
     return k_out, v_out
 
@@ -260,8 +272,7 @@ def gqa_decode_paged_fp8(q, k_cache, v_cache, scales, block_table, kv_lens, scal
     max_pages = block_table.shape[1]
     _want("block_table", block_table, torch.int32, (B, max_pages))
     _want("kv_lens", kv_lens, torch.int32, (B,))
-    _on_gpu(q=q, k_cache=k_cache, v_cache=v_cache, scales=scales, block_table=block_table, kv_lens=kv_lens,
-            workspace=workspace, out=out, lse=lse)
+    dev = _on_gpu(q, k_cache, v_cache, scales, block_table, kv_lens, workspace, out, lse)
     if out is None:
         out = torch.empty_like(q)
     else:
@@ -277,6 +288,7 @@ def gqa_decode_paged_fp8(q, k_cache, v_cache, scales, block_table, kv_lens, scal
     rc = _ffi.lib().bw_gqa_decode_paged_fp8(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr(), block_table.data_ptr(),
         kv_lens.data_ptr(), out.data_ptr(), lse.data_ptr(), B, Hq, Hkv, D, page_size, num_pages, max_pages,
-        float(scale if scale is not None else 1.0 / math.sqrt(D)), workspace.data_ptr(), workspace.nbytes, _stream())
+        float(scale if scale is not None else 1.0 / math.sqrt(D)), workspace.data_ptr(), workspace.nbytes,
+        _raw_stream(dev))
     _ffi.check(rc, "bw_gqa_decode_paged_fp8")
     return out, lse
