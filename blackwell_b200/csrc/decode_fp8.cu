@@ -213,19 +213,26 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
       const Segment sg = next_segment(p, prefix, t0, t1);
       const int* bt = p.block_table + (int64_t)sg.b * p.max_pages;
       const int last = ((sg.len - 1) / bh) * bh;   // pieces past the end read the last one again
-      auto row_of = [&](int t) -> int {            // first cache row of this lane's piece of the tile at t
-        const int tok = min(t + piece * bh, last);
-        const int pi = tok / p.page_size;
-        int page = bt[pi];
-        if ((unsigned)page >= (unsigned)p.num_pages) {
-          atomicCAS(p.err, 0, kErrIndexBit);
-          page = 0;
-        }
-        return page * p.page_size + (tok - pi * p.page_size);
-      };
-      int row = works ? row_of(sg.tok0) : 0;
+      const int last_page = last / p.page_size;
+      // Page indices: a lane holds one of 32 consecutive ones, and the next 32 are on their way.
+      int base = sg.tok0 / p.page_size;
+      int held = bt[min(base + lane, last_page)], next = bt[min(base + 32 + lane, last_page)];
       for (int t = sg.tok0; t < sg.tok1; t += kTile, ++n) {
         const uint32_t s = n % C::kStages;
+        const int tok = min(t + piece * bh, last);   // first token of this lane's piece
+        const int pi = tok / p.page_size, place = tok - pi * p.page_size;
+        if (__shfl_sync(0xffffffffu, pi, 0) >= base + 32) {   // lane 0 has the tile's first page
+          base += 32;
+          held = next;
+          next = bt[min(base + 32 + lane, last_page)];
+        }
+        // a tile's pages may reach into the next 32
+        const int in_held = __shfl_sync(0xffffffffu, held, pi - base), in_next = __shfl_sync(0xffffffffu, next, pi - base);
+        int page = pi - base < 32 ? in_held : in_next;
+        if ((unsigned)page >= (unsigned)p.num_pages) {
+          if (works) atomicCAS(p.err, 0, kErrIndexBit);
+          page = 0;
+        }
         bool got = true;
         if (lane == 0) {
           got = wc.wait(&bars.empty[s], ((n / C::kStages) & 1) ^ 1);
@@ -236,20 +243,19 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
           break;
         }
         if (works) {
+          const int row = page * p.page_size + place;
           uint8_t* dst = smem + s * C::kStage + piece * bh * D;
           if (kind == 0) {
             tma_load_2d(dst, &maps.k, &bars.full[s], kvh * D, row);
           } else if (kind == 1) {
             tma_load_2d(dst + C::kHalf, &maps.v, &bars.full[s], kvh * D, row);
           } else {
-            const int page = row / p.page_size, place = row - page * p.page_size;
             const uint8_t* src = p.scales + ((int64_t)page * p.Hkv + kvh) * 2 * p.page_size + place;
             const uint32_t to = sbase + C::kScales + s * 2 * kTile;
             if (one_copy) bulk_load(to + piece * 2 * bh, src, 2 * bh, &bars.full[s]);
             else if (kind == 2) bulk_load(to, src, kTile, &bars.full[s]);
             else bulk_load(to + kTile, src + p.page_size, kTile, &bars.full[s]);
           }
-          if (t + kTile < sg.tok1) row = row_of(t + kTile);   // its page index arrives while the ring is full
         }
       }
     }
