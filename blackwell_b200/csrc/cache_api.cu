@@ -306,6 +306,9 @@ int bw_gqa_decode_paged_fp8(const void* Q, const void* K_cache, const void* V_ca
   p.num_pages = num_pages;
   p.max_pages = max_pages_per_seq;
   p.max_tokens = (int)max_tokens;
+  p.page_shift = -1;
+  for (int i = 3; i < 31; ++i)
+    if (page_size == 1 << i) p.page_shift = i;
   p.scale_log2 = scale * 1.4426950408889634f;
   const int blocks = bw::decode_fp8_blocks(sms, D, G);
   p.groups = decode_groups(Hkv, blocks < kMaxDecodeBlocks ? blocks : kMaxDecodeBlocks);

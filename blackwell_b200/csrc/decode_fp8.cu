@@ -5,7 +5,7 @@
 //   o = sum_t p_t 2^ev_t v_t / sum_t p_t,  LSE = max x + ln sum_t p_t
 // with k_t, v_t the codes of token t.
 //
-// Split: the 64-token tiles of all sequences, one after the other, are dealt
+// Split: the tiles of all sequences, one after the other, are dealt
 // to `groups` token groups in equal contiguous runs, so the load is even
 // whatever the lengths are; a group has one block per KV head (the heads of a
 // token are neighbours in memory and are read at the same time).  A run meets
@@ -21,8 +21,12 @@
 namespace bw {
 namespace {
 
-constexpr int kTile = 64;      // tokens
-constexpr int kMinTiles = 4;   // tiles of a run, at least
+// Tokens of a tile: each consumer warp takes 16 U of it in one step (U
+// independent chains of products in flight).  Heads of 64 have half the bytes a
+// token and so twice the softmax per byte; U = 2 hides its latency.
+__host__ __device__ constexpr int units(int D) { return D == 128 ? 1 : 2; }
+__host__ __device__ constexpr int tile_tokens(int D) { return 64 * units(D); }
+constexpr int kMinTokens = 256;   // tokens of a run, at least
 constexpr int kWarps = 4;      // consumers
 constexpr int kThreads = 32 * (kWarps + 1);
 // Resident blocks an SM: registers (96 accumulators and Q fragments a thread in
@@ -37,6 +41,7 @@ __device__ __forceinline__ int seq_len(const Fp8DecodeParams& p, int b) {
 }
 
 // prefix[b] = tiles before sequence b (prefix[B] = all), by the whole block.
+template <int kTile>
 __device__ void tile_prefix(const Fp8DecodeParams& p, int* prefix, int* warp_sum) {
   const int tid = threadIdx.x, nth = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.B + nth - 1) / nth;
@@ -61,19 +66,21 @@ __device__ void tile_prefix(const Fp8DecodeParams& p, int* prefix, int* warp_sum
   __syncthreads();
 }
 
+template <int kTile>
 __device__ __forceinline__ int tiles_per_group(int total, int groups) {
-  return max((total + groups - 1) / groups, kMinTiles);
+  return max((total + groups - 1) / groups, kMinTokens / kTile);
 }
 
 // ------------------------------------------------------------------ shared memory of a block
-// A stage is one tile: K and V codes of 64 tokens (pieces of bh = min(64, page
-// size) rows, D bytes a row, 16-byte chunks swizzled by the tensor map) and the
-// scale bytes [piece][K, V][bh].
+// A stage is one tile: K and V codes (pieces of bh = min(64, page size) rows, D
+// bytes a row, 16-byte chunks swizzled by the tensor map) and the scale bytes of
+// K, then of V.
 template <int D>
 struct Cfg {
+  static constexpr int kTile = tile_tokens(D);
   static constexpr int kHalf = kTile * D;            // K (or V) codes of a stage
-  static constexpr int kStage = 2 * kHalf;
-  static constexpr int kStages = D == 128 ? 4 : 8;   // 64 KB in flight a block
+  static constexpr int kStage = 2 * kHalf;           // 16 KB
+  static constexpr int kStages = 4;
   static constexpr int kScales = kStages * kStage;
   static constexpr int kRed = kScales + kStages * 2 * kTile;    // m, l, M of 4 warps x 16 heads
   static constexpr int kBars = kRed + 3 * kWarps * 16 * 4;
@@ -122,17 +129,19 @@ __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
-// Untiled bulk copy of `bytes` (a multiple of 16, both addresses 16-byte aligned).
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
+// Asynchronous copy of N = 4 or 8 bytes; the thread's arrival on `bar` follows
+// when its copies so far have landed.
+template <int N>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, uint64_t* bar) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 struct Segment {
   int b, len, tok0, tok1;   // tokens [tok0, tok1) of sequence b
 };
 // The segment that begins at tile t0 of the run [t0, t1); t0 moves behind it.
+template <int kTile>
 __device__ __forceinline__ Segment next_segment(const Fp8DecodeParams& p, const int* prefix, int& t0, int t1) {
   int lo = 0, hi = p.B - 1;   // the last sequence that begins at or before t0, and so holds it
   while (lo < hi) {
@@ -150,7 +159,7 @@ __device__ __forceinline__ Segment next_segment(const Fp8DecodeParams& p, const 
 }
 
 // One producer warp streams the tiles of the block's run through a ring of
-// stages; four consumer warps take 16 tokens of a tile each, keep their own
+// stages; four consumer warps take 16 U tokens of a tile each, keep their own
 // running softmax and output, and merge at the end of a segment.
 //
 // The products run with tokens (then columns d) as the 16 rows of m16n8k16 and
@@ -174,6 +183,7 @@ template <int D, int NT>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
     decode_fp8_kernel(const Fp8DecodeParams p, const __grid_constant__ Fp8DecodeMaps maps) {
   using C = Cfg<D>;
+  constexpr int U = units(D), kTile = C::kTile;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Bars<D>& bars = *reinterpret_cast<Bars<D>*>(smem + C::kBars);
@@ -181,84 +191,80 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&bars.full[s], 1);
+      mbar_init(&bars.full[s], 1 + 32);   // the codes' byte count, and each producer lane's scale bytes
       mbar_init(&bars.empty[s], kWarps);
     }
     bars.abort_flag = 0;
     fence_mbar_init();
   }
-  tile_prefix(p, prefix, bars.warp_sum);   // synchronises the block
+  tile_prefix<kTile>(p, prefix, bars.warp_sum);   // synchronises the block
   asm volatile("griddepcontrol.launch_dependents;");
   const int grp = blockIdx.x / p.Hkv, kvh = blockIdx.x - grp * p.Hkv;
-  const int total = prefix[p.B], per = tiles_per_group(total, p.groups);
+  const int total = prefix[p.B], per = tiles_per_group<kTile>(total, p.groups);
   if (blockIdx.x == 0)
     for (int b = tid; b <= p.B; b += kThreads) p.prefix[b] = prefix[b];
   int t0 = min(grp * per, total);
   const int t1 = min(t0 + per, total);
   const WaitCtl wc{&bars.abort_flag, p.err, p.timeout_ns, 48 + warp};
   const uint32_t sbase = smem_u32(smem);
-  const int bh = p.page_size < kTile ? p.page_size : kTile;   // rows of a piece
+  const int bh = p.page_size < 64 ? p.page_size : 64;   // rows of a piece
 
   if (warp == kWarps) {
     // ------------------------------------------------------------ producer
-    // Lane = (piece of the tile, what of it): K codes, V codes, scale bytes (of K
-    // and V together in pages up to 64 tokens, else one lane each).
+    // The codes of a piece are two tensor copies (K, V), one lane each; a lane also
+    // copies the scale bytes of 4 U tokens (K: lanes 0-15, V: 16-31).
     const int np = kTile / bh;
     const int piece = lane % np, kind = lane / np;
-    const bool one_copy = p.page_size <= kTile;
-    const bool works = kind < (one_copy ? 3 : 4);
+    const auto page_of = [&](int tok) { return p.page_shift >= 0 ? tok >> p.page_shift : tok / p.page_size; };
     uint32_t n = 0;
     bool ok = true;
     while (ok && t0 < t1) {
-      const Segment sg = next_segment(p, prefix, t0, t1);
+      const Segment sg = next_segment<kTile>(p, prefix, t0, t1);
       const int* bt = p.block_table + (int64_t)sg.b * p.max_pages;
-      const int last = ((sg.len - 1) / bh) * bh;   // pieces past the end read the last one again
-      const int last_page = last / p.page_size;
+      // what lies past the end reads the last piece (the last scale bytes) again
+      const int last = ((sg.len - 1) / bh) * bh, last_sc = ((sg.len - 1) / (4 * U)) * (4 * U);
+      const int last_page = page_of(last);
       // Page indices: a lane holds one of 32 consecutive ones, and the next 32 are on their way.
-      int base = sg.tok0 / p.page_size;
+      int base = page_of(sg.tok0);
       int held = bt[min(base + lane, last_page)], next = bt[min(base + 32 + lane, last_page)];
       for (int t = sg.tok0; t < sg.tok1; t += kTile, ++n) {
         const uint32_t s = n % C::kStages;
-        const int tok = min(t + piece * bh, last);   // first token of this lane's piece
-        const int pi = tok / p.page_size, place = tok - pi * p.page_size;
-        if (__shfl_sync(0xffffffffu, pi, 0) >= base + 32) {   // lane 0 has the tile's first page
+        const int first = page_of(t);
+        if (first >= base + 32) {
           base += 32;
           held = next;
           next = bt[min(base + 32 + lane, last_page)];
         }
-        // a tile's pages may reach into the next 32
-        const int in_held = __shfl_sync(0xffffffffu, held, pi - base), in_next = __shfl_sync(0xffffffffu, next, pi - base);
-        int page = pi - base < 32 ? in_held : in_next;
-        if ((unsigned)page >= (unsigned)p.num_pages) {
-          if (works) atomicCAS(p.err, 0, kErrIndexBit);
-          page = 0;
-        }
+        const auto page_at = [&](int pi) {   // a tile's pages may reach into the next 32
+          const int a = __shfl_sync(0xffffffffu, held, pi - base), b = __shfl_sync(0xffffffffu, next, pi - base);
+          int page = pi - base < 32 ? a : b;
+          if ((unsigned)page >= (unsigned)p.num_pages) {
+            atomicCAS(p.err, 0, kErrIndexBit);
+            page = 0;
+          }
+          return page;
+        };
+        const int tok = min(t + piece * bh, last), pi = page_of(tok);
+        const int row = page_at(pi) * p.page_size + (tok - pi * p.page_size);
+        const int tok_sc = min(t + (lane & 15) * 4 * U, last_sc), pi_sc = page_of(tok_sc);
+        const uint8_t* src = p.scales + (((int64_t)page_at(pi_sc) * p.Hkv + kvh) * 2 + (lane >> 4)) * p.page_size +
+                             (tok_sc - pi_sc * p.page_size);
         bool got = true;
         if (lane == 0) {
           got = wc.wait(&bars.empty[s], ((n / C::kStages) & 1) ^ 1);
-          if (got) mbar_arrive_expect_tx(&bars.full[s], C::kStage + 2 * kTile);
+          if (got) mbar_arrive_expect_tx(&bars.full[s], C::kStage);
         }
         if (!__shfl_sync(0xffffffffu, got, 0)) {
           ok = false;
           break;
         }
-        if (works) {
-          const int row = page * p.page_size + place;
-          uint8_t* dst = smem + s * C::kStage + piece * bh * D;
-          if (kind == 0) {
-            tma_load_2d(dst, &maps.k, &bars.full[s], kvh * D, row);
-          } else if (kind == 1) {
-            tma_load_2d(dst + C::kHalf, &maps.v, &bars.full[s], kvh * D, row);
-          } else {
-            const uint8_t* src = p.scales + ((int64_t)page * p.Hkv + kvh) * 2 * p.page_size + place;
-            const uint32_t to = sbase + C::kScales + s * 2 * kTile;
-            if (one_copy) bulk_load(to + piece * 2 * bh, src, 2 * bh, &bars.full[s]);
-            else if (kind == 2) bulk_load(to, src, kTile, &bars.full[s]);
-            else bulk_load(to + kTile, src + p.page_size, kTile, &bars.full[s]);
-          }
-        }
+        uint8_t* dst = smem + s * C::kStage + piece * bh * D;
+        if (kind == 0) tma_load_2d(dst, &maps.k, &bars.full[s], kvh * D, row);
+        else if (kind == 1) tma_load_2d(dst + C::kHalf, &maps.v, &bars.full[s], kvh * D, row);
+        copy_async<4 * U>(sbase + C::kScales + s * 2 * kTile + lane * 4 * U, src, &bars.full[s]);
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
     if (!ok && lane == 0) {
       for (uint32_t i = n > C::kStages ? n - C::kStages : 0; i < n; ++i)   // loads already in flight
@@ -272,22 +278,15 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
   float* red_m = reinterpret_cast<float*>(smem + C::kRed);   // [warp][16]
   float* red_l = red_m + kWarps * 16;
   float* red_M = red_l + kWarps * 16;
-  // This lane's ldmatrix row: token (lane >> 3 & 1) * 8 + (lane & 7) of the warp's 16, chunk (lane >> 4) of a pair.
+  // This lane's ldmatrix row: token (lane >> 3 & 1) * 8 + (lane & 7) of a unit of 16, chunk (lane >> 4) of a pair.
   // 16-byte chunk c of tile row r lies at chunk c ^ (r & 7) of its row (128-byte rows), c ^ (r >> 1 & 3) (64-byte rows).
-  const int lrow = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+  const int lrow = warp * 16 * U + ((lane >> 3) & 1) * 8 + (lane & 7);
   const uint32_t row_off = (uint32_t)lrow * D;   // pieces follow one another: a row's place does not depend on bh
   const uint32_t swz = D == 128 ? (lrow & 7) : ((lrow >> 1) & 3);
   const uint32_t chunk0 = lane >> 4;
-  // scale bytes of tokens g and g + 8 of the warp's 16: K; V is bh further
-  uint32_t sc_off[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int tl = warp * 16 + g + 8 * i;
-    sc_off[i] = (uint32_t)(C::kScales + (tl / bh) * 2 * bh + tl % bh);
-  }
   uint32_t n = 0;
   while (t0 < t1) {
-    const Segment sg = next_segment(p, prefix, t0, t1);
+    const Segment sg = next_segment<kTile>(p, prefix, t0, t1);
     // Q of head (n tile) + g as f16, brought to [1, 2) by a power of two; columns in the codes' order
     uint32_t qb[NT][D / 16][2];
     float qs[NT][2];
@@ -334,61 +333,104 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
       // On a timeout the warp still goes through the merge below, so that the
       // barriers stay matched.
       if (!wc.wait(&bars.full[s], (n / C::kStages) & 1)) break;
-      const int left = sg.tok1 - (t + warp * 16);   // tokens of this warp that exist
+      const int left = sg.tok1 - (t + warp * 16 * U);   // tokens of this warp that exist
       if (left > 0) {
         const uint32_t kb = sbase + s * C::kStage + row_off, vb = kb + C::kHalf;
-        // S^T: two chains of products
-        float acc[NT][2][4];
+        // S^T of the U units; U = 1: in two chains of products
+        constexpr int kChains = U == 1 ? 2 : 1;
+        float acc[U][NT][kChains][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < D / 16; j += 2) {
-          uint32_t r[4];
-          ldsm_x4(kb + (((j + chunk0) ^ swz) << 4), r);
+            for (int i = 0; i < kChains; ++i)
+              acc[u][nt][i][0] = acc[u][nt][i][1] = acc[u][nt][i][2] = acc[u][nt][i][3] = 0.f;
+#pragma unroll
+        for (int j = 0; j < D / 16; j += 2)
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            uint32_t r[4];
+            ldsm_x4(kb + u * 16 * D + (((j + chunk0) ^ swz) << 4), r);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t a0, a1, a2, a3;
+              e4m3x4_to_f16x4(r[2 * i], a0, a2);
+              e4m3x4_to_f16x4(r[2 * i + 1], a1, a3);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma_f16(acc[u][nt][i % kChains], a0, a1, a2, a3, qb[nt][j + i][0], qb[nt][j + i][1]);
+            }
+          }
+        const uint8_t* sc = smem + C::kScales + s * 2 * kTile + warp * 16 * U + g;
+        float ks[U][2], ev[U][2];   // of tokens g and g + 8
+#pragma unroll
+        for (int u = 0; u < U; ++u)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            uint32_t a0, a1, a2, a3;
-            e4m3x4_to_f16x4(r[2 * i], a0, a2);
-            e4m3x4_to_f16x4(r[2 * i + 1], a1, a3);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt][i], a0, a1, a2, a3, qb[nt][j + i][0], qb[nt][j + i][1]);
+            ks[u][i] = __uint_as_float((uint32_t)sc[16 * u + 8 * i] << 23);
+            ev[u][i] = (float)((int)sc[kTile + 16 * u + 8 * i] - 127);
           }
+        uint32_t sel[U][2];   // bytes (t0 2g, t0 2g+1, t1 2g, t1 2g+1) -> (t0, t1) of 2g and of 2g + 1
+#pragma unroll
+        for (int u = 0; u < U; ++u) sel[u][0] = sel[u][1] = 0x3120u;
+        if (left < 16 * U) {
+          // A token past the end is picked as zero, whatever its codes are (a weight of 0 would not silence a NaN).
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int tl = 16 * u + 8 * i + 2 * q4;
+              sel[u][i] = (tl < left ? 0x0100u : 0x0404u) | (tl + 1 < left ? 0x3020u : 0x4040u);
+            }
         }
-        const uint8_t* sc = smem + s * 2 * kTile;
-        const uint32_t kb0 = sc[sc_off[0]], kb1 = sc[sc_off[1]], vb0 = sc[sc_off[0] + bh], vb1 = sc[sc_off[1] + bh];
-        const float ks0 = __uint_as_float(kb0 << 23), ks1 = __uint_as_float(kb1 << 23);
-        const float ev0 = (float)((int)vb0 - 127), ev1 = (float)((int)vb1 - 127);
-        const bool in0 = g < left, in1 = g + 8 < left;
-        uint32_t pb[NT][2];
+        uint32_t pb[U][NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float x[2][2], y[2][2];   // [head 2 q4 + j][token g + 8 i]
+          float x[2][2 * U];   // [head 2 q4 + j][token 16 u + 8 i + g]
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 2 * U; ++e) {
+              const int u = e / 2, i = e % 2;
+              float a = acc[u][nt][0][2 * i + j];
+              if constexpr (kChains == 2) a += acc[u][nt][1][2 * i + j];
+              x[j][e] = a * ks[u][i] * qs[nt][j];
+            }
+          if (left < 16 * U) {
+#pragma unroll
+            for (int e = 0; e < 2 * U; ++e)
+              if (8 * e + g >= left) x[0][e] = x[1][e] = -INFINITY;
+          }
+          float y[2][2 * U];
           bool moved = false;
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            x[j][0] = in0 ? (acc[nt][0][j] + acc[nt][1][j]) * ks0 * qs[nt][j] : -INFINITY;
-            x[j][1] = in1 ? (acc[nt][0][2 + j] + acc[nt][1][2 + j]) * ks1 * qs[nt][j] : -INFINITY;
-            const float mx = fmaxf(x[j][0], x[j][1]);
+            float mx = fmaxf(x[j][0], x[j][1]), my;
+#pragma unroll
+            for (int e = 2; e < 2 * U; ++e) mx = fmaxf(mx, x[j][e]);
             if (mx > m[nt][j] + 8.f) {
               l[nt][j] *= ex2f(m[nt][j] - mx);
               m[nt][j] = mx;
             }
             const float sub = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
-            l[nt][j] += ex2f(x[j][0] - sub) + ex2f(x[j][1] - sub);
-            y[j][0] = in0 ? x[j][0] + ev0 : -INFINITY;
-            y[j][1] = in1 ? x[j][1] + ev1 : -INFINITY;
-            moved |= fmaxf(y[j][0], y[j][1]) > M[nt][j] + 8.f;
+#pragma unroll
+            for (int e = 0; e < 2 * U; ++e) {
+              l[nt][j] += ex2f(x[j][e] - sub);
+              y[j][e] = x[j][e] + ev[e / 2][e % 2];
+              my = e ? fmaxf(my, y[j][e]) : y[j][e];
+            }
+            moved |= my > M[nt][j] + 8.f;
           }
           if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              float mx = fmaxf(y[j][0], y[j][1]);
+              float mx = M[nt][j];
+#pragma unroll
+              for (int e = 0; e < 2 * U; ++e) mx = fmaxf(mx, y[j][e]);
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              mx = fmaxf(mx, M[nt][j]);
               const float corr = mx == -INFINITY ? 1.f : ex2f(M[nt][j] - mx);
               M[nt][j] = mx;
 #pragma unroll
@@ -399,26 +441,25 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
             }
           }
           const float M0 = M[nt][0] == -INFINITY ? 0.f : M[nt][0], M1 = M[nt][1] == -INFINITY ? 0.f : M[nt][1];
-          pb[nt][0] = transpose8x8(f16x2(ex2f(y[0][0] - M0), ex2f(y[1][0] - M1)));
-          pb[nt][1] = transpose8x8(f16x2(ex2f(y[0][1] - M0), ex2f(y[1][1] - M1)));
+#pragma unroll
+          for (int e = 0; e < 2 * U; ++e)
+            pb[e / 2][nt][e % 2] = transpose8x8(f16x2(ex2f(y[0][e] - M0), ex2f(y[1][e] - M1)));
         }
-        // O^T: bytes (t0 2g, t0 2g+1, t1 2g, t1 2g+1) -> (t0, t1) of 2g and of 2g + 1; a token past the end is
-        // picked as zero, whatever its codes are (a weight of 0 would not silence a NaN)
-        const uint32_t sel0 = (2 * q4 < left ? 0x0100u : 0x0404u) | (2 * q4 + 1 < left ? 0x3020u : 0x4040u);
-        const uint32_t sel1 = (2 * q4 + 8 < left ? 0x0100u : 0x0404u) | (2 * q4 + 9 < left ? 0x3020u : 0x4040u);
 #pragma unroll
-        for (int c = 0; c < D / 16; c += 2) {
-          uint32_t r[4];
-          ldsm_x4_t(vb + (((c + chunk0) ^ swz) << 4), r);
+        for (int c = 0; c < D / 16; c += 2)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            uint32_t a0, a1, a2, a3;
-            e4m3x4_to_f16x4(__byte_perm(r[2 * i], 0, sel0), a0, a1);
-            e4m3x4_to_f16x4(__byte_perm(r[2 * i + 1], 0, sel1), a2, a3);
+          for (int u = 0; u < U; ++u) {
+            uint32_t r[4];
+            ldsm_x4_t(vb + u * 16 * D + (((c + chunk0) ^ swz) << 4), r);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][c + i], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+            for (int i = 0; i < 2; ++i) {
+              uint32_t a0, a1, a2, a3;
+              e4m3x4_to_f16x4(__byte_perm(r[2 * i], 0, sel[u][0]), a0, a1);
+              e4m3x4_to_f16x4(__byte_perm(r[2 * i + 1], 0, sel[u][1]), a2, a3);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][c + i], a0, a1, a2, a3, pb[u][nt][0], pb[u][nt][1]);
+            }
           }
-        }
       }
       // the last stage of a segment is kept for the merge
       if (t + kTile < sg.tok1) {
@@ -520,7 +561,7 @@ __global__ void __launch_bounds__(128) decode_fp8_join_kernel(const Fp8DecodePar
   asm volatile("griddepcontrol.wait;" ::: "memory");   // the segments are written
   const int hq = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int kvh = hq / p.G, g = hq - kvh * p.G;
-  const int first = p.prefix[b], last = p.prefix[b + 1], per = tiles_per_group(p.prefix[p.B], p.groups);
+  const int first = p.prefix[b], last = p.prefix[b + 1], per = tiles_per_group<tile_tokens(D)>(p.prefix[p.B], p.groups);
   const int64_t row = (int64_t)b * p.Hq + hq;
   __nv_bfloat16* O = static_cast<__nv_bfloat16*>(p.O) + row * D;
   if (first == last) {                       // no tokens

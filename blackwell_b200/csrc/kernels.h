@@ -215,7 +215,8 @@ struct Fp8DecodeParams {
   void* O;                   // bf16 [B, Hq, D]
   float* LSE;                // fp32 [B, Hq] or null
   int B, Hq, Hkv, G, D, page_size, num_pages, max_pages;
-  int max_tokens;            // max_pages * page_size, at most 2^31 - 64
+  int max_tokens;            // max_pages * page_size, at most 2^30
+  int page_shift;            // log2(page_size), -1 where it is no power of two
   int groups;                // token groups; groups * Hkv blocks
   float scale_log2;
   float* o_part;             // [(groups + B) * Hkv, G, D] fp32
