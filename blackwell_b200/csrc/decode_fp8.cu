@@ -24,14 +24,14 @@ namespace {
 // Tokens of a tile: each consumer warp takes 16 U of it in one step (U
 // independent chains of products in flight).  Heads of 64 have half the bytes a
 // token and so twice the softmax per byte; U = 2 hides its latency.
-__host__ __device__ constexpr int units(int D) { return D == 128 ? 1 : 2; }
+__host__ __device__ constexpr int units(int D) { return D == 128 ? 2 : 4; }
 __host__ __device__ constexpr int tile_tokens(int D) { return 64 * units(D); }
 constexpr int kMinTokens = 256;   // tokens of a run, at least
-constexpr int kWarps = 4;      // consumers
-constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kWarps = 4;      // consumers; one producer warp more for K and one for V
+constexpr int kThreads = 32 * (kWarps + 2);
 // Resident blocks an SM: registers (96 accumulators and Q fragments a thread in
 // the largest variant) and shared memory (about 67 KB a block).
-constexpr int blocks_per_sm(int D, int NT) { return D == 128 && NT == 2 ? 2 : 3; }
+constexpr int blocks_per_sm(int D, int NT) { return 2; }
 
 // Tokens of sequence b: kv_lens[b], at least 0 and at most what its row of the
 // block table can hold.
@@ -80,7 +80,7 @@ struct Cfg {
   static constexpr int kTile = tile_tokens(D);
   static constexpr int kHalf = kTile * D;            // K (or V) codes of a stage
   static constexpr int kStage = 2 * kHalf;           // 16 KB
-  static constexpr int kStages = 4;
+  static constexpr int kStages = 3;
   static constexpr int kScales = kStages * kStage;
   static constexpr int kRed = kScales + kStages * 2 * kTile;    // m, l, M of 4 warps x 16 heads
   static constexpr int kBars = kRed + 3 * kWarps * 16 * 4;
@@ -129,7 +129,7 @@ __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
-// Asynchronous copy of N = 4 or 8 bytes; the thread's arrival on `bar` follows
+// Asynchronous copy of N = 4, 8 or 16 bytes; the thread's arrival on `bar` follows
 // when its copies so far have landed.
 template <int N>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, uint64_t* bar) {
@@ -184,6 +184,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
     decode_fp8_kernel(const Fp8DecodeParams p, const __grid_constant__ Fp8DecodeMaps maps) {
   using C = Cfg<D>;
   constexpr int U = units(D), kTile = C::kTile;
+  constexpr int kScaleBytes = kTile / 32;   // of K (or V), a producer lane
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Bars<D>& bars = *reinterpret_cast<Bars<D>*>(smem + C::kBars);
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&bars.full[s], 1 + 32);   // the codes' byte count, and each producer lane's scale bytes
+      mbar_init(&bars.full[s], 2 * (1 + 32));   // of either producer: the codes' byte count, each lane's scale bytes
       mbar_init(&bars.empty[s], kWarps);
     }
     bars.abort_flag = 0;
@@ -209,12 +210,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
   const uint32_t sbase = smem_u32(smem);
   const int bh = p.page_size < 64 ? p.page_size : 64;   // rows of a piece
 
-  if (warp == kWarps) {
-    // ------------------------------------------------------------ producer
-    // The codes of a piece are two tensor copies (K, V), one lane each; a lane also
-    // copies the scale bytes of 4 U tokens (K: lanes 0-15, V: 16-31).
+  if (warp >= kWarps) {
+    // ------------------------------------------------------------ producers
+    // One warp copies K, one V: a tensor copy a piece, one lane each (the
+    // hardware takes them from a warp one after the other, which is why there
+    // are two warps), and the scale bytes of 2 U tokens by every lane.
+    const int is_v = warp - kWarps;
+    const CUtensorMap* map = is_v ? &maps.v : &maps.k;
     const int np = kTile / bh;
-    const int piece = lane % np, kind = lane / np;
     const auto page_of = [&](int tok) { return p.page_shift >= 0 ? tok >> p.page_shift : tok / p.page_size; };
     uint32_t n = 0;
     bool ok = true;
@@ -222,15 +225,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
       const Segment sg = next_segment<kTile>(p, prefix, t0, t1);
       const int* bt = p.block_table + (int64_t)sg.b * p.max_pages;
       // what lies past the end reads the last piece (the last scale bytes) again
-      const int last = ((sg.len - 1) / bh) * bh, last_sc = ((sg.len - 1) / (4 * U)) * (4 * U);
+      const int last = ((sg.len - 1) / bh) * bh, last_sc = ((sg.len - 1) / kScaleBytes) * kScaleBytes;
       const int last_page = page_of(last);
       // Page indices: a lane holds one of 32 consecutive ones, and the next 32 are on their way.
       int base = page_of(sg.tok0);
       int held = bt[min(base + lane, last_page)], next = bt[min(base + 32 + lane, last_page)];
       for (int t = sg.tok0; t < sg.tok1; t += kTile, ++n) {
         const uint32_t s = n % C::kStages;
-        const int first = page_of(t);
-        if (first >= base + 32) {
+        if (page_of(t) >= base + 32) {
           base += 32;
           held = next;
           next = bt[min(base + 32 + lane, last_page)];
@@ -244,24 +246,22 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
           }
           return page;
         };
-        const int tok = min(t + piece * bh, last), pi = page_of(tok);
+        const int tok = min(t + (lane < np ? lane : 0) * bh, last), pi = page_of(tok);
         const int row = page_at(pi) * p.page_size + (tok - pi * p.page_size);
-        const int tok_sc = min(t + (lane & 15) * 4 * U, last_sc), pi_sc = page_of(tok_sc);
-        const uint8_t* src = p.scales + (((int64_t)page_at(pi_sc) * p.Hkv + kvh) * 2 + (lane >> 4)) * p.page_size +
+        const int tok_sc = min(t + lane * kScaleBytes, last_sc), pi_sc = page_of(tok_sc);
+        const uint8_t* src = p.scales + (((int64_t)page_at(pi_sc) * p.Hkv + kvh) * 2 + is_v) * p.page_size +
                              (tok_sc - pi_sc * p.page_size);
         bool got = true;
         if (lane == 0) {
           got = wc.wait(&bars.empty[s], ((n / C::kStages) & 1) ^ 1);
-          if (got) mbar_arrive_expect_tx(&bars.full[s], C::kStage);
+          if (got) mbar_arrive_expect_tx(&bars.full[s], C::kHalf);
         }
         if (!__shfl_sync(0xffffffffu, got, 0)) {
           ok = false;
           break;
         }
-        uint8_t* dst = smem + s * C::kStage + piece * bh * D;
-        if (kind == 0) tma_load_2d(dst, &maps.k, &bars.full[s], kvh * D, row);
-        else if (kind == 1) tma_load_2d(dst + C::kHalf, &maps.v, &bars.full[s], kvh * D, row);
-        copy_async<4 * U>(sbase + C::kScales + s * 2 * kTile + lane * 4 * U, src, &bars.full[s]);
+        if (lane < np) tma_load_2d(smem + s * C::kStage + is_v * C::kHalf + lane * bh * D, map, &bars.full[s], kvh * D, row);
+        copy_async<kScaleBytes>(sbase + C::kScales + (s * 2 + is_v) * kTile + lane * kScaleBytes, src, &bars.full[s]);
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
