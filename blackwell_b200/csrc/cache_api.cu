@@ -149,8 +149,9 @@ int bw_rope(const void* Q, void* Q_out, const void* K, void* K_out, int dtype, i
   p.S = S;
   p.D = D;
   p.R = rotary_dim;
-  p.units = rotary_dim / 16;
-  if (!in_place(p.q) || (K && !in_place(p.k))) p.units += (D - rotary_dim + 15) / 16;
+  // two vectors of 16 bytes a thread; behind the rotary part only where something is to be copied
+  p.units = rotary_dim / (2 * mult);
+  if (!in_place(p.q) || (K && !in_place(p.k))) p.units += ((D - rotary_dim) / mult + 1) / 2;
   p.fp32 = dtype == BW_F32;
   p.half = interleaved ? 0 : 1;
   p.inverse = inverse ? 1 : 0;

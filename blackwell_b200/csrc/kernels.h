@@ -159,7 +159,7 @@ struct RopeTensor {
 struct RopeParams {
   RopeTensor q, k;
   int B, S, D, R;
-  int units;                 // threads per token: R / 16 and the pass-through ones (0 in place)
+  int units;                 // threads per token: the rotary ones and (out of place) those behind
   int fp32;                  // 1: fp32 tensors, 0: bf16
   int half;                  // 1: pairs (i, i + R/2); 0: pairs (2i, 2i + 1)
   int inverse;

@@ -7,6 +7,8 @@
 // Slot = page * page_size + place in the page.
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "kernels.h"
 #include "rope_math.cuh"
 
@@ -16,8 +18,8 @@ namespace {
 constexpr int kThreads = 256;
 
 // Rows (token, KV head, K or V) one after the other, D / 16 lanes a row, 16
-// elements a lane: the two chunks of 8 that rotate among themselves
-// (half layout: 8 sub and R/2 + 8 sub), or 16 consecutive elements.
+// elements a lane: two chunks of 8 in the rotary part, R / 2 apart, or 16
+// consecutive elements.
 template <int D, bool FP8, bool ROPE, bool HALF>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvWriteParams p) {
   constexpr int LPR = D / 16;
@@ -42,7 +44,7 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvWriteParams 
   bool turns = false;
   if constexpr (ROPE) {
     turns = !is_v && sub < (p.R >> 4);
-    if (HALF && turns) {
+    if (turns) {
       e0 = 8 * sub;
       e1 = e0 + (p.R >> 1);
     }
@@ -62,10 +64,10 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvWriteParams 
       const int64_t pos = p.positions[t];
       if (pos >= 0 && pos < p.table_len) {
         float c[8], sn[8];
-        const float* cs = p.table + pos * p.R + 8 * sub;
-        load8(cs, c);
-        load8(cs + (p.R >> 1), sn);
-        rotate16<HALF>(x, c, sn);
+        const float* cs = p.table + pos * p.R;
+        load_angles<8, HALF>(cs, e0, e1, c);
+        load_angles<8, HALF>(cs + (p.R >> 1), e0, e1, sn);
+        rotate<8, HALF>(x, c, sn);
         raw[0] = f32_to_bf16x8(x);
         raw[1] = f32_to_bf16x8(x + 8);
       }
@@ -108,11 +110,16 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvWriteParams 
   }
 }
 
-// blockIdx.y = sequence; threads walk its (token, 16-element unit of the
-// [Hkv, D] row), K and V together.
+// blockIdx.y = sequence; a block takes kReadTokens tokens at a time.  Its threads
+// walk the (token, 8-element unit) pairs of them, kUnroll pairs of K and V loads
+// in flight a thread; neighbouring threads write neighbouring 16 bytes, so every
+// store covers whole sectors.
+constexpr int kReadTokens = 16, kUnroll = 4;
+
 template <int D, bool FP8>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvReadParams p) {
-  constexpr int LPR = D / 16;
+  constexpr int LPR = D / 8;
+  using Raw = typename std::conditional<FP8, uint2, uint4>::type;   // 8 elements
   const int b = blockIdx.y;
   const int len = p.kv_lens[b];
   if (len <= 0) return;
@@ -122,46 +129,57 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvReadParams p)
     if (blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(p.err, 0, kErrIndexBit);
     return;
   }
-  const int upr = p.Hkv * LPR;   // units a token
-  const int64_t n = (int64_t)len * upr;
+  const uint32_t upr = (uint32_t)p.Hkv * LPR;   // units a token
   const int* bt = p.block_table + (int64_t)b * p.max_pages;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
-    const int64_t tok = i / upr;
-    const int unit = (int)(i - tok * upr);
-    const int at = (int)(start + tok);
-    const int pi = at / p.page_size, place = at - pi * p.page_size;
-    const int page = bt[pi];
-    if (page < 0 || page >= p.num_pages) {
-      atomicCAS(p.err, 0, kErrIndexBit);
-      continue;
-    }
-    const int64_t src = ((int64_t)page * p.page_size + place) * p.Hkv * D + 16 * unit;
-    const int64_t dst = (out0 + tok) * p.Hkv * D + 16 * unit;
+  for (int tok0 = blockIdx.x * kReadTokens; tok0 < len; tok0 += gridDim.x * kReadTokens) {
+    const uint32_t n = (uint32_t)min(kReadTokens, len - tok0) * upr;
+    for (uint32_t i0 = threadIdx.x; i0 < n; i0 += kThreads * kUnroll) {
+      Raw raw[kUnroll][2];
+      uint8_t sc[kUnroll][2];
+      int64_t dst[kUnroll];
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const void* cache = w ? p.v_cache : p.k_cache;
-      uint4* out = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(w ? p.v_out : p.k_out) + dst);
-      if constexpr (FP8) {
-        const uint4 c = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(cache) + src);
-        const int h = unit / LPR;
-        const float sc = __uint_as_float(
-            (uint32_t)p.scales[(((int64_t)page * p.Hkv + h) * 2 + w) * p.page_size + place] << 23);
-        const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
-        uint32_t o[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float f[4];
-          e4m3x4_to_f32(cw[j], f);
-          o[2 * j] = f32_to_bf16x2(f[0] * sc, f[1] * sc);
-          o[2 * j + 1] = f32_to_bf16x2(f[2] * sc, f[3] * sc);
+      for (int u = 0; u < kUnroll; ++u) {
+        const uint32_t i = i0 + u * kThreads;
+        dst[u] = -1;
+        if (i >= n) continue;
+        const uint32_t tok = i / upr, unit = i - tok * upr;
+        const uint32_t at = (uint32_t)start + tok0 + tok;
+        const uint32_t pi = at / (uint32_t)p.page_size, place = at - pi * p.page_size;
+        const int page = bt[pi];
+        if ((unsigned)page >= (unsigned)p.num_pages) {
+          atomicCAS(p.err, 0, kErrIndexBit);
+          continue;
         }
-        out[0] = make_uint4(o[0], o[1], o[2], o[3]);
-        out[1] = make_uint4(o[4], o[5], o[6], o[7]);
-      } else {
-        const uint4* in = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(cache) + src);
-        const uint4 a = in[0], c = in[1];
-        out[0] = a;
-        out[1] = c;
+        const int64_t src = ((int64_t)page * p.page_size + place) * p.Hkv * D + 8 * unit;
+        dst[u] = (out0 + tok0 + tok) * p.Hkv * D + 8 * unit;
+        const int64_t esz = FP8 ? 1 : 2;
+        raw[u][0] = *reinterpret_cast<const Raw*>(static_cast<const uint8_t*>(p.k_cache) + src * esz);
+        raw[u][1] = *reinterpret_cast<const Raw*>(static_cast<const uint8_t*>(p.v_cache) + src * esz);
+        if constexpr (FP8) {
+          const uint8_t* s = p.scales + ((int64_t)page * p.Hkv + unit / LPR) * 2 * p.page_size + place;
+          sc[u][0] = s[0];
+          sc[u][1] = s[p.page_size];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        if (dst[u] < 0) continue;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          uint4 o;
+          if constexpr (FP8) {
+            const float scale = __uint_as_float((uint32_t)sc[u][w] << 23);
+            float f[8];
+            e4m3x4_to_f32(raw[u][w].x, f);
+            e4m3x4_to_f32(raw[u][w].y, f + 4);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] *= scale;
+            o = f32_to_bf16x8(f);
+          } else {
+            o = raw[u][w];
+          }
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(w ? p.v_out : p.k_out) + dst[u]) = o;
+        }
       }
     }
   }
@@ -191,11 +209,11 @@ cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream) {
 
 cudaError_t launch_kv_read(const KvReadParams& p, int num_sms, cudaStream_t stream) {
   // Blocks for the longest span that the table's width or the output's rows
-  // allow, at most about 8 resident blocks' worth on every SM over all sequences.
+  // allow, at most about 16 an SM over all sequences.
   int64_t most = (int64_t)p.max_pages * p.page_size;
   if (most > p.total_rows) most = p.total_rows;
-  int64_t bx = (most * p.Hkv * (p.D / 16) + kThreads - 1) / kThreads;
-  const int64_t cap = ((int64_t)num_sms * 8 + p.B - 1) / p.B;
+  int64_t bx = (most + kReadTokens - 1) / kReadTokens;
+  const int64_t cap = ((int64_t)num_sms * 16 + p.B - 1) / p.B;
   if (bx > cap) bx = cap;
   const dim3 grid((unsigned)bx, (unsigned)p.B);
   if (p.D == 128) {

@@ -19,20 +19,27 @@ namespace bw {
 namespace {
 
 // One thread owns one pair (its frequency stays in a register) and walks rows.
-// The angle is kept in turns and in fp64 until only the quarter turn around it
-// is left: p f / 2 pi has an absolute error near p f 2^-53, so positions of
-// millions keep full fp32 accuracy; |rest| <= 1/2 quarter turn goes to fp32.
+// The angle is kept in quarter turns and in fp64 until only the part around the
+// nearest whole number of them is left: p f has an absolute error near p f 2^-52,
+// so positions of millions keep full fp32 accuracy; the rest, at most half a
+// quarter turn, goes to fp32.  Adding 1.5 * 2^52 rounds to a whole number whose
+// low bits are the quadrant, which saves the conversions between fp64 and
+// integers.  Bound by the stores.
 __global__ void rope_table_kernel(const RopeTableParams p) {
+  constexpr double kRound = 6755399441055744.0;   // 1.5 * 2^52
   const int i = threadIdx.x;
   const int half = p.R >> 1;
-  const double f = p.turns[i];
-  for (int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; r < p.length; r += (int64_t)gridDim.x * blockDim.y) {
-    const double quarters = 4.0 * (f * (double)(p.first + r));
-    const double whole = rint(quarters);
-    const float rest = (float)(quarters - whole);
+  const double f = 4.0 * p.turns[i];
+  int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  const int64_t step = (int64_t)gridDim.x * blockDim.y;
+  double pos = (double)(p.first + r);
+  for (; r < p.length; r += step, pos += (double)step) {
+    const double quarters = f * pos;
+    const double whole = quarters + kRound;
+    const float rest = (float)(quarters - (whole - kRound));
     float s, c;
     sincospif(0.5f * rest, &s, &c);
-    const int q = (int)((long long)whole & 3);
+    const int q = __double2loint(whole) & 3;
     float cc = (q & 1) ? s : c, ss = (q & 1) ? c : s;   // turn by q quarters
     if (q == 1 || q == 2) cc = -cc;
     if (q >= 2) ss = -ss;
@@ -42,42 +49,34 @@ __global__ void rope_table_kernel(const RopeTableParams p) {
   }
 }
 
+// 16 bytes of a head: V elements.
 template <typename T>
-struct Chunk8;   // eight consecutive elements
+struct Vec;
 template <>
-struct Chunk8<__nv_bfloat16> {
-  uint4 v;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void store(__nv_bfloat16* p) const { *reinterpret_cast<uint4*>(p) = v; }
-  __device__ __forceinline__ void get(float* x) const { bf16x8_to_f32(v, x); }
-  __device__ __forceinline__ void set(const float* x) { v = f32_to_bf16x8(x); }
+struct Vec<__nv_bfloat16> {
+  static constexpr int V = 8;
+  static __device__ __forceinline__ void get(const uint4& v, float* x) { bf16x8_to_f32(v, x); }
+  static __device__ __forceinline__ uint4 set(const float* x) { return f32_to_bf16x8(x); }
 };
 template <>
-struct Chunk8<float> {
-  float4 a, b;
-  __device__ __forceinline__ void load(const float* p) {
-    a = *reinterpret_cast<const float4*>(p);
-    b = *reinterpret_cast<const float4*>(p + 4);
+struct Vec<float> {
+  static constexpr int V = 4;
+  static __device__ __forceinline__ void get(const uint4& v, float* x) {
+    x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
   }
-  __device__ __forceinline__ void store(float* p) const {
-    *reinterpret_cast<float4*>(p) = a;
-    *reinterpret_cast<float4*>(p + 4) = b;
-  }
-  __device__ __forceinline__ void get(float* x) const {
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  }
-  __device__ __forceinline__ void set(const float* x) {
-    a = make_float4(x[0], x[1], x[2], x[3]);
-    b = make_float4(x[4], x[5], x[6], x[7]);
+  static __device__ __forceinline__ uint4 set(const float* x) {
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
   }
 };
 
-// A thread owns one unit of a token: 16 elements that rotate among themselves
-// (two chunks of 8: c0 = 8u and c0 + R/2, or 16u and 16u + 8), or two chunks
-// behind the rotary part.  It reads its 8 cos and 8 sin once and applies them
-// to kHeads heads, whose loads are all in flight together.
+// A thread owns one unit of a token: two vectors of 16 bytes, R / 2 elements
+// apart, that rotate with each other (half layout) or each within itself, or two
+// vectors behind the rotary part; neighbouring threads read neighbouring
+// vectors.  It reads its cos and sin once and applies them to kHeads heads, whose
+// loads are all in flight together.
 template <typename T, bool HALF, int kHeads>
 __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
+  constexpr int V = Vec<T>::V;
   const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const int64_t tok = idx / p.units;
   if (tok >= (int64_t)p.B * p.S) return;
@@ -89,46 +88,47 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
   const T* in = static_cast<const T*>(t.in) + b * t.in_sb + s * t.in_ss + h0 * t.in_sh;
   T* out = static_cast<T*>(t.out) + b * t.out_sb + s * t.out_ss + h0 * t.out_sh;
 
-  const int rot = p.R >> 4;   // rotary units
+  const int rot = p.R / (2 * V);   // rotary units
   const bool turns = unit < rot;
-  const int e0 = turns ? (HALF ? 8 * unit : 16 * unit) : p.R + 16 * (unit - rot);
-  const int e1 = turns ? (HALF ? 8 * unit + (p.R >> 1) : 16 * unit + 8) : e0 + 8;
-  const bool two = e1 < p.D;   // D - R may be an odd number of chunks
-  Chunk8<T> x[kHeads][2];
+  const int rest = (p.D - p.R) / V;   // vectors behind the rotary part
+  const int e0 = turns ? V * unit : p.R + V * (unit - rot);
+  const int e1 = turns ? e0 + (p.R >> 1) : e0 + V * ((rest + 1) / 2);
+  const bool two = e1 < p.D;
+  uint4 x[kHeads][2];
 #pragma unroll
   for (int u = 0; u < kHeads; ++u)
     if (h0 + u < t.H) {
-      x[u][0].load(in + u * t.in_sh + e0);
-      if (two) x[u][1].load(in + u * t.in_sh + e1);
+      x[u][0] = *reinterpret_cast<const uint4*>(in + u * t.in_sh + e0);
+      if (two) x[u][1] = *reinterpret_cast<const uint4*>(in + u * t.in_sh + e1);
     }
   if (turns) {
     const int64_t pos = (int64_t)(p.positions ? p.positions[tok] : s) + p.pos_offset;
     if (pos >= 0 && pos < p.table_len) {
-      float c[8], sn[8];
-      const float* cs = p.table + pos * p.R + 8 * unit;
-      load8(cs, c);
-      load8(cs + (p.R >> 1), sn);
+      float c[V], sn[V];
+      const float* cs = p.table + pos * p.R;
+      load_angles<V, HALF>(cs, e0, e1, c);
+      load_angles<V, HALF>(cs + (p.R >> 1), e0, e1, sn);
       if (p.inverse) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sn[i] = -sn[i];
+        for (int i = 0; i < V; ++i) sn[i] = -sn[i];
       }
 #pragma unroll
       for (int u = 0; u < kHeads; ++u)
         if (h0 + u < t.H) {
-          float y[16];
-          x[u][0].get(y);
-          x[u][1].get(y + 8);
-          rotate16<HALF>(y, c, sn);
-          x[u][0].set(y);
-          x[u][1].set(y + 8);
+          float y[2 * V];
+          Vec<T>::get(x[u][0], y);
+          Vec<T>::get(x[u][1], y + V);
+          rotate<V, HALF>(y, c, sn);
+          x[u][0] = Vec<T>::set(y);
+          x[u][1] = Vec<T>::set(y + V);
         }
     }
   }
 #pragma unroll
   for (int u = 0; u < kHeads; ++u)
     if (h0 + u < t.H) {
-      x[u][0].store(out + u * t.out_sh + e0);
-      if (two) x[u][1].store(out + u * t.out_sh + e1);
+      *reinterpret_cast<uint4*>(out + u * t.out_sh + e0) = x[u][0];
+      if (two) *reinterpret_cast<uint4*>(out + u * t.out_sh + e1) = x[u][1];
     }
 }
 
@@ -158,7 +158,7 @@ cudaError_t launch_rope_table(const RopeTableParams& p, int num_sms, cudaStream_
 }
 
 cudaError_t launch_rope(const RopeParams& p, cudaStream_t stream) {
-  return p.fp32 ? launch<float, 2>(p, stream) : launch<__nv_bfloat16, 4>(p, stream);
+  return p.fp32 ? launch<float, 4>(p, stream) : launch<__nv_bfloat16, 4>(p, stream);
 }
 
 }  // namespace bw

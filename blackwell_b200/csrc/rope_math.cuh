@@ -1,5 +1,5 @@
-// What the rotary and the cache kernels share: 16-byte conversions, the
-// rotation of 16 elements, and the 8-bit rows of the quantised cache.
+// What the rotary and the cache kernels share: 16-byte conversions, the rotation
+// of two vectors, and the 8-bit rows of the quantised cache.
 #pragma once
 #include <cstdint>
 #include <cuda_bf16.h>
@@ -23,20 +23,35 @@ __device__ __forceinline__ uint4 f32_to_bf16x8(const float* x) {
   return make_uint4(f32_to_bf16x2(x[0], x[1]), f32_to_bf16x2(x[2], x[3]), f32_to_bf16x2(x[4], x[5]),
                     f32_to_bf16x2(x[6], x[7]));
 }
-__device__ __forceinline__ void load8(const float* p, float* x) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p + 4));
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+__device__ __forceinline__ float4 ldg4(const float* p) { return __ldg(reinterpret_cast<const float4*>(p)); }
+
+// The V angles (cos or sin part of a table row) of two vectors of V elements at
+// e0 and e1 = e0 + R / 2: pairs (i, i + R/2) share the V angles e0 .., pairs
+// (2i, 2i + 1) have V / 2 from e0 / 2 and V / 2 from e1 / 2.
+template <int V, bool HALF>
+__device__ __forceinline__ void load_angles(const float* row, int e0, int e1, float* x) {
+  if constexpr (V == 8) {
+    const float4 a = ldg4(row + (HALF ? e0 : e0 / 2)), b = ldg4(row + (HALF ? e0 + 4 : e1 / 2));
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  } else if constexpr (HALF) {
+    const float4 a = ldg4(row + e0);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+  } else {
+    const float2 a = __ldg(reinterpret_cast<const float2*>(row + e0 / 2));
+    const float2 b = __ldg(reinterpret_cast<const float2*>(row + e1 / 2));
+    x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+  }
 }
 
-// Rotates 16 elements by 8 angles: pairs (i, i + 8) of the array (HALF) or
+// Rotates 2 V elements by V angles: pairs (i, i + V) of the array (HALF) or
 // (2i, 2i + 1).  Each product is rounded to fp32 by itself, so that the result
 // does not depend on which product a compiler contracts into an FMA: the fused
 // write of a rotated K row and the stand-alone rotation agree to the bit.
-template <bool HALF>
-__device__ __forceinline__ void rotate16(float (&x)[16], const float (&c)[8], const float (&s)[8]) {
+template <int V, bool HALF>
+__device__ __forceinline__ void rotate(float* x, const float* c, const float* s) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int ia = HALF ? i : 2 * i, ib = HALF ? i + 8 : 2 * i + 1;
+  for (int i = 0; i < V; ++i) {
+    const int ia = HALF ? i : 2 * i, ib = HALF ? i + V : 2 * i + 1;
     const float a = x[ia], b = x[ib];
     x[ia] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
     x[ib] = __fadd_rn(__fmul_rn(a, s[i]), __fmul_rn(b, c[i]));
