@@ -14,6 +14,9 @@
 // merges in segment order, so results do not depend on timing.
 #include <cuda_bf16.h>
 
+#include <atomic>
+
+#include "early_launch.cuh"
 #include "kernels.h"
 #include "ptx.cuh"
 #include "rope_math.cuh"
@@ -27,6 +30,7 @@ namespace {
 __host__ __device__ constexpr int units(int D) { return D == 128 ? 2 : 4; }
 __host__ __device__ constexpr int tile_tokens(int D) { return 64 * units(D); }
 constexpr int kMinTokens = 256;   // tokens of a run, at least
+constexpr int kMaxB = 4096;
 constexpr int kWarps = 4;      // consumers; one producer warp more for K and one for V
 constexpr int kThreads = 32 * (kWarps + 2);
 // Resident blocks an SM: registers (96 accumulators and Q fragments a thread in
@@ -198,8 +202,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
     bars.abort_flag = 0;
     fence_mbar_init();
   }
+  after_previous_kernel();
+  let_next_kernel_start();
   tile_prefix<kTile>(p, prefix, bars.warp_sum);   // synchronises the block
-  asm volatile("griddepcontrol.launch_dependents;");
   const int grp = blockIdx.x / p.Hkv, kvh = blockIdx.x - grp * p.Hkv;
   const int total = prefix[p.B], per = tiles_per_group<kTile>(total, p.groups);
   if (blockIdx.x == 0)
@@ -558,7 +563,7 @@ __global__ void __launch_bounds__(128) decode_fp8_join_kernel(const Fp8DecodePar
   constexpr int kRows = 128 / kLanes;        // segments in flight
   __shared__ float4 part[kRows][kLanes];
   __shared__ float wsum_s[kRows], max_s[4];
-  asm volatile("griddepcontrol.wait;" ::: "memory");   // the segments are written
+  after_previous_kernel();   // the segments are written
   const int hq = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int kvh = hq / p.G, g = hq - kvh * p.G;
   const int first = p.prefix[b], last = p.prefix[b + 1], per = tiles_per_group<tile_tokens(D)>(p.prefix[p.B], p.groups);
@@ -612,23 +617,19 @@ template <int D, int NT>
 cudaError_t launch(const Fp8DecodeParams& p, const Fp8DecodeMaps& maps, cudaStream_t stream) {
   auto kern = decode_fp8_kernel<D, NT>;
   const int bytes = Cfg<D>::kPrefix + (p.B + 1) * 4 + 1024;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  // Once per device; the limit, not what a launch takes, so it covers every B.
+  static std::atomic<uint64_t> allowed{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  kern<<<p.groups * p.Hkv, kThreads, bytes, stream>>>(p, maps);
-  e = cudaGetLastError();
+  if (dev >= 64 || !(allowed.load() >> dev & 1)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kPrefix + (kMaxB + 1) * 4 + 1024);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) allowed |= uint64_t(1) << dev;
+  }
+  e = launch_early(kern, dim3(p.groups * p.Hkv), dim3(kThreads), bytes, stream, p, maps);
   if (e != cudaSuccess) return e;
-  // The join's blocks start while the decode's last ones finish and wait there
-  // for its results (griddepcontrol), which takes the launch out of the path.
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.Hq, p.B);
-  cfg.blockDim = dim3(128);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, decode_fp8_join_kernel<D>, p);
+  return launch_early(decode_fp8_join_kernel<D>, dim3(p.Hq, p.B), dim3(128), 0, stream, p);
 }
 
 }  // namespace

@@ -9,6 +9,7 @@
 
 #include <type_traits>
 
+#include "early_launch.cuh"
 #include "kernels.h"
 #include "rope_math.cuh"
 
@@ -23,6 +24,7 @@ constexpr int kThreads = 256;
 template <int D, bool FP8, bool ROPE, bool HALF>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvWriteParams p) {
   constexpr int LPR = D / 16;
+  after_previous_kernel();
   const int64_t idx = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   const int64_t rows = (int64_t)p.T * p.Hkv * 2;
   int64_t row = idx / LPR;
@@ -121,6 +123,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvReadParams p)
   constexpr int LPR = D / 8;
   using Raw = typename std::conditional<FP8, uint2, uint4>::type;   // 8 elements
   const int b = blockIdx.y;
+  after_previous_kernel();
   const int len = p.kv_lens[b];
   if (len <= 0) return;
   const int64_t start = p.kv_starts ? p.kv_starts[b] : 0;
@@ -186,25 +189,20 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvReadParams p)
 }
 
 template <int D, bool FP8>
-void write_launch(const KvWriteParams& p, cudaStream_t stream) {
+cudaError_t write_launch(const KvWriteParams& p, cudaStream_t stream) {
   const int64_t threads = (int64_t)p.T * p.Hkv * 2 * (D / 16);
-  const unsigned blocks = (unsigned)((threads + kThreads - 1) / kThreads);
-  if (p.table == nullptr) kv_write_kernel<D, FP8, false, false><<<blocks, kThreads, 0, stream>>>(p);
-  else if (p.half) kv_write_kernel<D, FP8, true, true><<<blocks, kThreads, 0, stream>>>(p);
-  else kv_write_kernel<D, FP8, true, false><<<blocks, kThreads, 0, stream>>>(p);
+  const dim3 blocks((unsigned)((threads + kThreads - 1) / kThreads));
+  auto kern = p.table == nullptr ? kv_write_kernel<D, FP8, false, false>
+              : p.half           ? kv_write_kernel<D, FP8, true, true>
+                                 : kv_write_kernel<D, FP8, true, false>;
+  return launch_early(kern, blocks, dim3(kThreads), 0, stream, p);
 }
 
 }  // namespace
 
 cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream) {
-  if (p.D == 128) {
-    if (p.fp8) write_launch<128, true>(p, stream);
-    else write_launch<128, false>(p, stream);
-  } else {
-    if (p.fp8) write_launch<64, true>(p, stream);
-    else write_launch<64, false>(p, stream);
-  }
-  return cudaGetLastError();
+  if (p.D == 128) return p.fp8 ? write_launch<128, true>(p, stream) : write_launch<128, false>(p, stream);
+  return p.fp8 ? write_launch<64, true>(p, stream) : write_launch<64, false>(p, stream);
 }
 
 cudaError_t launch_kv_read(const KvReadParams& p, int num_sms, cudaStream_t stream) {
@@ -215,15 +213,9 @@ cudaError_t launch_kv_read(const KvReadParams& p, int num_sms, cudaStream_t stre
   int64_t bx = (most + kReadTokens - 1) / kReadTokens;
   const int64_t cap = ((int64_t)num_sms * 16 + p.B - 1) / p.B;
   if (bx > cap) bx = cap;
-  const dim3 grid((unsigned)bx, (unsigned)p.B);
-  if (p.D == 128) {
-    if (p.fp8) kv_read_kernel<128, true><<<grid, kThreads, 0, stream>>>(p);
-    else kv_read_kernel<128, false><<<grid, kThreads, 0, stream>>>(p);
-  } else {
-    if (p.fp8) kv_read_kernel<64, true><<<grid, kThreads, 0, stream>>>(p);
-    else kv_read_kernel<64, false><<<grid, kThreads, 0, stream>>>(p);
-  }
-  return cudaGetLastError();
+  auto kern = p.D == 128 ? (p.fp8 ? kv_read_kernel<128, true> : kv_read_kernel<128, false>)
+                         : (p.fp8 ? kv_read_kernel<64, true> : kv_read_kernel<64, false>);
+  return launch_early(kern, dim3((unsigned)bx, (unsigned)p.B), dim3(kThreads), 0, stream, p);
 }
 
 }  // namespace bw

@@ -12,6 +12,7 @@
 // through unchanged, as in bw_qk_norm_rope.
 #include <cuda_bf16.h>
 
+#include "early_launch.cuh"
 #include "kernels.h"
 #include "rope_math.cuh"
 
@@ -30,15 +31,19 @@ __global__ void rope_table_kernel(const RopeTableParams p) {
   const int i = threadIdx.x;
   const int half = p.R >> 1;
   const double f = 4.0 * p.turns[i];
+  after_previous_kernel();
   int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
   double pos = (double)(p.first + r);
   for (; r < p.length; r += step, pos += (double)step) {
     const double quarters = f * pos;
     const double whole = quarters + kRound;
-    const float rest = (float)(quarters - (whole - kRound));
-    float s, c;
-    sincospif(0.5f * rest, &s, &c);
+    const float x = (float)((quarters - (whole - kRound)) * 1.5707963267948966);   // |x| <= pi / 4
+    const float x2 = x * x;
+    // Taylor series; the terms left out are below 2^-28 of sin x and 2^-32 of cos x at pi / 4
+    const float s = fmaf(x * x2, fmaf(x2, fmaf(x2, fmaf(x2, 1.f / 362880.f, -1.f / 5040.f), 1.f / 120.f), -1.f / 6.f), x);
+    const float c = fmaf(
+        x2, fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, -1.f / 3628800.f, 1.f / 40320.f), -1.f / 720.f), 1.f / 24.f), -0.5f), 1.f);
     const int q = __double2loint(whole) & 3;
     float cc = (q & 1) ? s : c, ss = (q & 1) ? c : s;   // turn by q quarters
     if (q == 1 || q == 2) cc = -cc;
@@ -77,6 +82,7 @@ struct Vec<float> {
 template <typename T, bool HALF, int kHeads>
 __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
   constexpr int V = Vec<T>::V;
+  after_previous_kernel();
   const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const int64_t tok = idx / p.units;
   if (tok >= (int64_t)p.B * p.S) return;
@@ -140,9 +146,8 @@ cudaError_t launch(RopeParams p, cudaStream_t stream) {
   // Few tokens: small blocks, so that the work spreads over the SMs.
   const int block = threads <= 148 * 64 ? 64 : 256;
   const dim3 grid((unsigned)((threads + block - 1) / block), (unsigned)(p.q_groups + k_groups));
-  if (p.half) rope_kernel<T, true, kHeads><<<grid, block, 0, stream>>>(p);
-  else rope_kernel<T, false, kHeads><<<grid, block, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_early(p.half ? rope_kernel<T, true, kHeads> : rope_kernel<T, false, kHeads>, grid, dim3(block), 0,
+                      stream, p);
 }
 
 }  // namespace
@@ -153,8 +158,7 @@ cudaError_t launch_rope_table(const RopeTableParams& p, int num_sms, cudaStream_
   int64_t blocks = (p.length + block.y - 1) / block.y;
   const int64_t cap = (int64_t)num_sms * 8;
   if (blocks > cap) blocks = cap;
-  rope_table_kernel<<<(unsigned)blocks, block, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_early(rope_table_kernel, dim3((unsigned)blocks), block, 0, stream, p);
 }
 
 cudaError_t launch_rope(const RopeParams& p, cudaStream_t stream) {
