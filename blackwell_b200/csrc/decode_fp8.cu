@@ -29,7 +29,6 @@ namespace {
 // token and so twice the softmax per byte; U = 2 hides its latency.
 __host__ __device__ constexpr int units(int D) { return D == 128 ? 2 : 4; }
 __host__ __device__ constexpr int tile_tokens(int D) { return 64 * units(D); }
-constexpr int kMinTokens = 256;   // tokens of a run, at least
 constexpr int kMaxB = 4096;
 constexpr int kWarps = 4;      // consumers; one producer warp more for K and one for V
 constexpr int kThreads = 32 * (kWarps + 2);
@@ -70,10 +69,7 @@ __device__ void tile_prefix(const Fp8DecodeParams& p, int* prefix, int* warp_sum
   __syncthreads();
 }
 
-template <int kTile>
-__device__ __forceinline__ int tiles_per_group(int total, int groups) {
-  return max((total + groups - 1) / groups, kMinTokens / kTile);
-}
+__device__ __forceinline__ int tiles_per_group(int total, int groups) { return max((total + groups - 1) / groups, 1); }
 
 // ------------------------------------------------------------------ shared memory of a block
 // A stage is one tile: K and V codes (pieces of bh = min(64, page size) rows, D
@@ -202,11 +198,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
     bars.abort_flag = 0;
     fence_mbar_init();
   }
+  if (warp >= kWarps && lane == 0) prefetch_tmap(warp == kWarps ? &maps.k : &maps.v);
   after_previous_kernel();
   let_next_kernel_start();
   tile_prefix<kTile>(p, prefix, bars.warp_sum);   // synchronises the block
   const int grp = blockIdx.x / p.Hkv, kvh = blockIdx.x - grp * p.Hkv;
-  const int total = prefix[p.B], per = tiles_per_group<kTile>(total, p.groups);
+  const int total = prefix[p.B], per = tiles_per_group(total, p.groups);
   if (blockIdx.x == 0)
     for (int b = tid; b <= p.B; b += kThreads) p.prefix[b] = prefix[b];
   int t0 = min(grp * per, total);
@@ -555,22 +552,23 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
   }
 }
 
-// One block per (sequence, query head): the segments of the sequence are the
-// groups whose runs meet its tiles.
-template <int D>
-__global__ void __launch_bounds__(128) decode_fp8_join_kernel(const Fp8DecodeParams p) {
+// One block of T threads per (sequence, query head): the segments of the sequence
+// are the groups whose runs meet its tiles; kUnroll times the segments that fit
+// side by side are in flight.
+template <int D, int T, int kUnroll>
+__global__ void __launch_bounds__(T) decode_fp8_join_kernel(const Fp8DecodeParams p) {
   constexpr int kLanes = D / 4;              // 4 columns a thread
-  constexpr int kRows = 128 / kLanes;        // segments in flight
+  constexpr int kRows = T / kLanes;          // segments side by side
   __shared__ float4 part[kRows][kLanes];
-  __shared__ float wsum_s[kRows], max_s[4];
+  __shared__ float wsum_s[kRows], max_s[T / 32];
   after_previous_kernel();   // the segments are written
   const int hq = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int kvh = hq / p.G, g = hq - kvh * p.G;
-  const int first = p.prefix[b], last = p.prefix[b + 1], per = tiles_per_group<tile_tokens(D)>(p.prefix[p.B], p.groups);
+  const int first = p.prefix[b], last = p.prefix[b + 1], per = tiles_per_group(p.prefix[p.B], p.groups);
   const int64_t row = (int64_t)b * p.Hq + hq;
   __nv_bfloat16* O = static_cast<__nv_bfloat16*>(p.O) + row * D;
   if (first == last) {                       // no tokens
-    for (int d = tid; d < D; d += 128) O[d] = __float2bfloat16(0.f);
+    for (int d = tid; d < D; d += T) O[d] = __float2bfloat16(0.f);
     if (p.LSE && tid == 0) p.LSE[row] = -INFINITY;
     return;
   }
@@ -578,24 +576,39 @@ __global__ void __launch_bounds__(128) decode_fp8_join_kernel(const Fp8DecodePar
   if (n == 1) return;                        // written by its segment
   const int64_t base = ((int64_t)(g0 + b) * p.Hkv + kvh) * p.G + g, step = (int64_t)p.Hkv * p.G;
   float mx = -INFINITY;
-  for (int i = tid; i < n; i += 128) mx = fmaxf(mx, p.lse_part[base + i * step]);
+  for (int i = tid; i < n; i += T) mx = fmaxf(mx, p.lse_part[base + i * step]);
 #pragma unroll
   for (int off = 16; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
   if ((tid & 31) == 0) max_s[tid >> 5] = mx;
   __syncthreads();
-  mx = fmaxf(fmaxf(max_s[0], max_s[1]), fmaxf(max_s[2], max_s[3]));
+#pragma unroll
+  for (int w = 0; w < T / 32; ++w) mx = fmaxf(mx, max_s[w]);
   const float sub = mx == -INFINITY ? 0.f : mx;
   const int lane = tid % kLanes, r = tid / kLanes;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float wsum = 0.f;
-  for (int i = r; i < n; i += kRows) {
-    const float w = __expf(p.lse_part[base + i * step] - sub);
-    const float4 v = *reinterpret_cast<const float4*>(p.o_part + (base + i * step) * D + 4 * lane);
-    wsum += w;
-    acc.x = fmaf(w, v.x, acc.x);
-    acc.y = fmaf(w, v.y, acc.y);
-    acc.z = fmaf(w, v.z, acc.z);
-    acc.w = fmaf(w, v.w, acc.w);
+  for (int i0 = r; i0 < n; i0 += kRows * kUnroll) {
+    float w[kUnroll];
+    float4 v[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int i = i0 + u * kRows;
+      w[u] = -INFINITY;
+      if (i < n) {
+        w[u] = p.lse_part[base + i * step];
+        v[u] = *reinterpret_cast<const float4*>(p.o_part + (base + i * step) * D + 4 * lane);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (i0 + u * kRows < n) {
+        const float e = __expf(w[u] - sub);
+        wsum += e;
+        acc.x = fmaf(e, v[u].x, acc.x);
+        acc.y = fmaf(e, v[u].y, acc.y);
+        acc.z = fmaf(e, v[u].z, acc.z);
+        acc.w = fmaf(e, v[u].w, acc.w);
+      }
   }
   part[r][lane] = acc;
   if (lane == 0) wsum_s[r] = wsum;
@@ -629,7 +642,14 @@ cudaError_t launch(const Fp8DecodeParams& p, const Fp8DecodeMaps& maps, cudaStre
   }
   e = launch_early(kern, dim3(p.groups * p.Hkv), dim3(kThreads), bytes, stream, p, maps);
   if (e != cudaSuccess) return e;
-  return launch_early(decode_fp8_join_kernel<D>, dim3(p.Hq, p.B), dim3(128), 0, stream, p);
+  // A sequence has about groups / B segments, and no more than tiles.  Many (few KV
+  // heads, few long sequences): wide blocks with 4 loads in flight a thread (131072
+  // tokens, one KV head, 256 segments: 18.9 us for both kernels against 26).  Few:
+  // the small kernel starts sooner (one sequence of 517 tokens: 7.6 against 8.0 us;
+  // 32 of 500 to 2000: 24.3 against 25.4).
+  if (p.groups > 32 * p.B && p.max_tokens > 32 * Cfg<D>::kTile)
+    return launch_early(decode_fp8_join_kernel<D, 512, 4>, dim3(p.Hq, p.B), dim3(512), 0, stream, p);
+  return launch_early(decode_fp8_join_kernel<D, 128, 1>, dim3(p.Hq, p.B), dim3(128), 0, stream, p);
 }
 
 }  // namespace
