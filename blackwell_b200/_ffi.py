@@ -10,6 +10,7 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libbw_attn.so"
+FRONT_PATH = Path(__file__).resolve().parent / "_front.so"   # torch front end of cache.py
 
 (BW_OK, BW_ERR_SHAPE, BW_ERR_ALIGN, BW_ERR_CUDA, BW_ERR_TIMEOUT, BW_ERR_NCCL, BW_ERR_NULL, BW_ERR_WORKSPACE,
  BW_ERR_INDEX) = range(9)

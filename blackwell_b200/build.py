@@ -2,8 +2,9 @@
 
     python -m blackwell_b200.build        # -> blackwell_b200/libbw_attn.so
 
-It also links the C++ harness ``bw_harness`` (harness/bw_harness.cpp) against
-the library.  Every .cu under csrc/ is compiled with
+It also links the C++ harness ``bw_harness`` (harness/bw_harness.cpp) and the
+torch front end of the cache calls ``_front.so`` (front/front.cpp, a CPython
+module) against the library.  Every .cu under csrc/ is compiled with
 ``-gencode arch=compute_100a,code=sm_100a -lineinfo -O3`` and linked into one
 shared library with the CUDA runtime linked statically (no torch types cross
 the boundary; the library only depends on the driver at run time).
@@ -21,6 +22,8 @@ CSRC = HERE / "csrc"
 OUT = HERE / "libbw_attn.so"
 HARNESS = HERE / "bw_harness"
 HARNESS_SRC = HERE / "harness" / "bw_harness.cpp"
+FRONT = HERE / "_front.so"
+FRONT_SRC = HERE / "front" / "front.cpp"
 BUILD = HERE / "_build"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -36,10 +39,10 @@ def _deps():
 
 
 def up_to_date() -> bool:
-    if not OUT.exists() or not HARNESS.exists():
+    if not OUT.exists() or not HARNESS.exists() or not FRONT.exists():
         return False
-    t = min(OUT.stat().st_mtime, HARNESS.stat().st_mtime)
-    return all(p.stat().st_mtime <= t for p in _deps() + [HARNESS_SRC])
+    t = min(OUT.stat().st_mtime, HARNESS.stat().st_mtime, FRONT.stat().st_mtime)
+    return all(p.stat().st_mtime <= t for p in _deps() + [HARNESS_SRC, FRONT_SRC])
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -62,7 +65,31 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     subprocess.run(cmd, check=True)
     os.replace(tmp, OUT)
     build_harness(verbose)
+    build_front(verbose)
     return OUT
+
+
+def build_front(verbose: bool = False) -> Path:
+    """The torch front end: a CPython module over the C ABI, linked to the library."""
+    import shutil
+    import sysconfig
+
+    import torch
+    cuda = Path(shutil.which(NVCC) or NVCC).resolve().parent.parent
+    root = Path(torch.__file__).resolve().parent
+    tmp = FRONT.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for p in (root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
+              cuda / "include", sysconfig.get_paths()["include"]):
+        cmd += ["-isystem", str(p)]
+    cmd += [str(FRONT_SRC), "-o", str(tmp), "-L", str(HERE), "-lbw_attn", "-Wl,-rpath,$ORIGIN",
+            "-L", str(root / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, FRONT)
+    return FRONT
 
 
 def build_harness(verbose: bool = False) -> Path:
