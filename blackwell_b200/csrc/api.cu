@@ -234,13 +234,14 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 namespace bw {
 
-int device_info(void* stream, int* num_sms, int** err, uint64_t* timeout_ns) {
+int device_info(void* stream, DeviceInfo* info) {
   DeviceState* dev = nullptr;
   const int rc = get_device_state(&dev);
   if (rc != BW_OK) return rc;
-  *num_sms = dev->num_sms;
-  *err = err_slot(dev, stream);
-  *timeout_ns = (uint64_t)g_timeout_ns.load();
+  info->num_sms = dev->num_sms;
+  info->err = err_slot(dev, stream);
+  info->timeout_ns = (uint64_t)g_timeout_ns.load();
+  info->debug_flags = (int)g_debug_flags.load();
   return BW_OK;
 }
 

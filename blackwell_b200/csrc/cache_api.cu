@@ -116,16 +116,15 @@ int bw_rope_table(float* table, int64_t length, int rotary_dim, int64_t first, c
   double magnitude = 1.0;
   int rc = schedule(rotary_dim, scaling, p.turns, &magnitude);
   if (rc != BW_OK) return rc;
-  int sms = 0, *err = nullptr;
-  uint64_t ns = 0;
-  rc = bw::device_info(stream, &sms, &err, &ns);
+  bw::DeviceInfo dev;
+  rc = bw::device_info(stream, &dev);
   if (rc != BW_OK) return rc;
   p.table = table;
   p.length = length;
   p.first = first;
   p.R = rotary_dim;
   p.magnitude = (float)magnitude;
-  return bw::launch_rope_table(p, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? BW_OK : BW_ERR_CUDA;
+  return bw::launch_rope_table(p, dev.num_sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? BW_OK : BW_ERR_CUDA;
 }
 
 int bw_rope(const void* Q, void* Q_out, const void* K, void* K_out, int dtype, int B, int Hq, int Hkv, int S, int D,
@@ -159,9 +158,8 @@ int bw_rope(const void* Q, void* Q_out, const void* K, void* K_out, int dtype, i
   p.table_len = cache_seq_len;
   p.positions = positions;
   p.pos_offset = pos_offset;
-  int sms = 0, *err = nullptr;
-  uint64_t ns = 0;
-  rc = bw::device_info(stream, &sms, &err, &ns);
+  bw::DeviceInfo dev;
+  rc = bw::device_info(stream, &dev);
   if (rc != BW_OK) return rc;
   return bw::launch_rope(p, static_cast<cudaStream_t>(stream)) == cudaSuccess ? BW_OK : BW_ERR_CUDA;
 }
@@ -212,10 +210,10 @@ int bw_kv_cache_write(const void* K, const void* V, const int64_t* k_strides, co
   p.R = rotary_dim;
   p.half = interleaved ? 0 : 1;
   p.positions = positions;
-  int sms = 0;
-  uint64_t ns = 0;
-  const int rc = bw::device_info(stream, &sms, &p.err, &ns);
+  bw::DeviceInfo dev;
+  const int rc = bw::device_info(stream, &dev);
   if (rc != BW_OK) return rc;
+  p.err = dev.err;
   return bw::launch_kv_write(p, static_cast<cudaStream_t>(stream)) == cudaSuccess ? BW_OK : BW_ERR_CUDA;
 }
 
@@ -254,11 +252,11 @@ int bw_kv_cache_read(const void* K_cache, const void* V_cache, const uint8_t* sc
   p.num_pages = num_pages;
   p.max_pages = max_pages_per_seq;
   p.fp8 = cache_dtype == BW_E4M3;
-  int sms = 0;
-  uint64_t ns = 0;
-  const int rc = bw::device_info(stream, &sms, &p.err, &ns);
+  bw::DeviceInfo dev;
+  const int rc = bw::device_info(stream, &dev);
   if (rc != BW_OK) return rc;
-  return bw::launch_kv_read(p, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? BW_OK : BW_ERR_CUDA;
+  p.err = dev.err;
+  return bw::launch_kv_read(p, dev.num_sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? BW_OK : BW_ERR_CUDA;
 }
 
 size_t bw_gqa_decode_paged_fp8_workspace_size(int B, int Hq, int Hkv, int D) {
@@ -287,9 +285,12 @@ int bw_gqa_decode_paged_fp8(const void* Q, const void* K_cache, const void* V_ca
     return BW_ERR_ALIGN;
   if (workspace_bytes < bw_gqa_decode_paged_fp8_workspace_size(B, Hq, Hkv, D)) return BW_ERR_WORKSPACE;
   bw::Fp8DecodeParams p{};
-  int sms = 0;
-  const int rc = bw::device_info(stream, &sms, &p.err, &p.timeout_ns);
+  bw::DeviceInfo dev;
+  const int rc = bw::device_info(stream, &dev);
   if (rc != BW_OK) return rc;
+  p.err = dev.err;
+  p.timeout_ns = dev.timeout_ns;
+  p.debug_flags = dev.debug_flags;
   p.Q = Q;
   p.k_cache = K_cache;
   p.v_cache = V_cache;
@@ -311,7 +312,7 @@ int bw_gqa_decode_paged_fp8(const void* Q, const void* K_cache, const void* V_ca
   for (int i = 3; i < 31; ++i)
     if (page_size == 1 << i) p.page_shift = i;
   p.scale_log2 = scale * 1.4426950408889634f;
-  const int blocks = bw::decode_fp8_blocks(sms, D, G);
+  const int blocks = bw::decode_fp8_blocks(dev.num_sms, D, G);
   p.groups = decode_groups(Hkv, blocks < kMaxDecodeBlocks ? blocks : kMaxDecodeBlocks);
   bw::Fp8DecodeMaps maps;
   const int64_t rows = (int64_t)num_pages * page_size;

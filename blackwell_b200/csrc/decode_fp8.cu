@@ -30,6 +30,7 @@ namespace {
 __host__ __device__ constexpr int units(int D) { return D == 128 ? 2 : 4; }
 __host__ __device__ constexpr int tile_tokens(int D) { return 64 * units(D); }
 constexpr int kMaxB = 4096;
+constexpr uint64_t kDrainNs = 20000000;   // 20 ms, thousands of times what a copy takes
 constexpr int kWarps = 4;      // consumers; one producer warp more for K and one for V
 constexpr int kThreads = 32 * (kWarps + 2);
 // Resident blocks an SM: registers (96 accumulators and Q fragments a thread in
@@ -262,15 +263,19 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
           ok = false;
           break;
         }
-        if (lane < np) tma_load_2d(smem + s * C::kStage + is_v * C::kHalf + lane * bh * D, map, &bars.full[s], kvh * D, row);
+        const bool withheld = (p.debug_flags & 1) && !is_v && n == 0;
+        if (lane < np && !withheld)
+          tma_load_2d(smem + s * C::kStage + is_v * C::kHalf + lane * bh * D, map, &bars.full[s], kvh * D, row);
         copy_async<kScaleBytes>(sbase + C::kScales + (s * 2 + is_v) * kTile + lane * kScaleBytes, src, &bars.full[s]);
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
     if (!ok && lane == 0) {
-      for (uint32_t i = n > C::kStages ? n - C::kStages : 0; i < n; ++i)   // loads already in flight
-        drain_wait(&bars.full[i % C::kStages], (i / C::kStages) & 1, p.timeout_ns);
+      // Copies in flight must land before the block gives its memory back.  A stage
+      // that the other producer no longer filled stays open: the bound ends it.
+      for (uint32_t i = n > C::kStages ? n - C::kStages : 0; i < n; ++i)
+        drain_wait(&bars.full[i % C::kStages], (i / C::kStages) & 1, kDrainNs);
     }
     return;
   }
@@ -334,7 +339,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
       s = n % C::kStages;
       // On a timeout the warp still goes through the merge below, so that the
       // barriers stay matched.
-      if (!wc.wait(&bars.full[s], (n / C::kStages) & 1)) break;
+      const bool got = wc.wait(&bars.full[s], (n / C::kStages) & 1);
+      if (!__all_sync(0xffffffffu, got)) break;   // the warp decides as one
       const int left = sg.tok1 - (t + warp * 16 * U);   // tokens of this warp that exist
       if (left > 0) {
         const uint32_t kb = sbase + s * C::kStage + row_off, vb = kb + C::kHalf;
@@ -547,8 +553,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
     if (tid == 0) bars.stop = *wc.abort_flag;
     fence_proxy_async_smem();   // the stage goes back to the copies
     consumer_sync();
+    if (*(volatile int*)&bars.stop) break;   // and no stage is given back any more
     if (lane == 0) mbar_arrive(&bars.empty[s]);
-    if (*(volatile int*)&bars.stop) break;
   }
 }
 

@@ -224,6 +224,7 @@ struct Fp8DecodeParams {
   int* prefix;               // [B + 1]
   int* err;
   uint64_t timeout_ns;
+  int debug_flags;           // bit 0: the K producer withholds its first tile (timeout test)
 };
 struct Fp8DecodeMaps {
   // 2-D (Hkv * D, rows) bytes over K or V codes; box (D, min(64, page_size)),
@@ -238,8 +239,15 @@ cudaError_t launch_decode_fp8(const Fp8DecodeParams& p, const Fp8DecodeMaps& map
 int make_map_bytes(CUtensorMap* m, const void* base, int64_t row_bytes, int64_t rows, int box_bytes, int box_rows);
 
 // What an entry point outside api.cu needs of the current device: SM count, the
-// error word of `stream`, the bound on device-side waits.  Returns a status code.
-int device_info(void* stream, int* num_sms, int** err, uint64_t* timeout_ns);
+// error word of `stream`, the bound on device-side waits, the debug flags.  Returns
+// a status code.
+struct DeviceInfo {
+  int num_sms;
+  int* err;
+  uint64_t timeout_ns;
+  int debug_flags;
+};
+int device_info(void* stream, DeviceInfo* info);
 
 // The attention forward of the C ABI with the internal extras: causal query
 // offset (multiple of 128) and LSE head stride (0 = Sq).  Returns a status code.

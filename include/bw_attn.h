@@ -296,7 +296,7 @@ BW_API int bw_kv_cache_write(const void* K, const void* V, const int64_t* k_stri
  * layout of bw_gqa_decode and, through strides, of bw_gqa_causal_offset_fwd (a
  * chunk's attention over its prefix).  Values are code * 2^e, exact in bf16
  * (beyond its range: infinity).  Rows that no span covers are left as they
- * are.  A span outside the block table or the output, and a token whose page is
+ * are; two spans may not share rows; a length of 0 or less reads nothing.  A span outside the block table or the output, and a token whose page is
  * outside the cache, are skipped and reported as BW_ERR_INDEX. */
 BW_API int bw_kv_cache_read(const void* K_cache, const void* V_cache, const uint8_t* scales, int cache_dtype,
                             int page_size, int num_pages, const int* block_table, int max_pages_per_seq,
@@ -307,12 +307,14 @@ BW_API int bw_kv_cache_read(const void* K_cache, const void* V_cache, const uint
  * V_cache e4m3, scales): same meaning of every argument, without `chunk`: the
  * tokens of all sequences are dealt evenly over the GPU, whatever their
  * lengths, and the parts of a sequence are merged by a second kernel.  Keys and
- * values enter at their exact values, Q is bf16, products and sums fp32; a
- * token's weight is rounded to fp16 (relative 2^-11 of the largest weight * value
- * scale).  O bf16, LSE natural log or NULL; a sequence without tokens gives
- * O = 0 and LSE = -inf.  Codes, scales and table entries past kv_lens[b] are
- * not used, whatever they hold.  A length beyond the table is cut to it.  A page
- * outside the cache reads as page 0 and is reported as BW_ERR_INDEX.
+ * values enter at their exact values, products are of fp16 and summed in fp32: Q is
+ * exact there down to 2^-14 of its row's largest element, and a token's weight
+ * times its value scale is rounded to fp16 (2^-11 of itself, 2^-25 of the largest
+ * one of the sequence's part below that).  O bf16, LSE natural log or NULL; a
+ * sequence without tokens gives O = 0 and LSE = -inf.  O and LSE may not overlap
+ * an input.  Codes, scales and table entries past kv_lens[b] are not used,
+ * whatever they hold.  A length beyond the table is cut to it.  A page outside
+ * the cache reads as page 0 and is reported as BW_ERR_INDEX.
  * Workspace: bw_gqa_decode_paged_fp8_workspace_size(B, Hq, Hkv, D) bytes, 16-byte
  * aligned, nothing in it needs a value before the call; calls that may overlap
  * need one each. */
@@ -351,9 +353,10 @@ BW_API int bw_stream_status(void* stream);
 
 /* Library options (process-wide).  Keys:
  *   BW_OPT_TIMEOUT_NS      bound on every device-side wait (default 2e9)
- *   BW_OPT_DEBUG_FLAGS     test hook; bit 0 makes the prefill producer withhold
- *                          its first K tile so that the consumers' bounded waits
- *                          expire and the call reports BW_ERR_TIMEOUT
+ *   BW_OPT_DEBUG_FLAGS     test hook; bit 0 makes the prefill producer (and the
+ *                          one of bw_gqa_decode_paged_fp8) withhold its first K
+ *                          tile so that the consumers' bounded waits expire and
+ *                          the call reports BW_ERR_TIMEOUT
  *   BW_OPT_MAX_CTAS        cap on the persistent prefill grid (0 = SM count)
  *   BW_OPT_EXP_POLY        of every 8 pairs of softmax exponentials, how many
  *                          are computed by an FMA-pipe polynomial instead of

@@ -225,3 +225,72 @@ def test_decode_fp8_in_graphs_and_on_streams():
     torch.cuda.synchronize()
     for x, (o, l, _) in zip(qs, outs):
         check(o, l, x.cpu(), codes, sc, bt, lens)
+
+
+@pytest.mark.parametrize("ps", [192, 320])
+def test_decode_fp8_pages_that_are_no_power_of_two(ps):
+    import blackwell_b200 as bw
+    lens = [ps, ps + 1, 2 * ps - 1, 1000]
+    for D in (64, 128):
+        q, codes, sc, bt = make(lens, 2, 4, D, ps, 81)
+        o, lse = run(q, codes, sc, bt, lens)
+        assert bw.stream_status() == 0
+        check(o, lse, q, codes, sc, bt, lens)
+
+
+@pytest.mark.parametrize("D,B", [(128, 4096), (64, 4096)])
+def test_decode_fp8_most_sequences(D, B):
+    """The largest batch: its tile counts take the most shared memory."""
+    import blackwell_b200 as bw
+    lens = list(np.random.default_rng(1).integers(0, 20, B))
+    q, codes, sc, bt = make(lens, 1, 2, D, 8, 91)
+    o, lse = run(q, codes, sc, bt, lens)
+    assert bw.stream_status() == 0
+    some = [0, 1, 77, B - 2, B - 1]
+    check(o[some], lse[some], q[some], codes, sc, bt[some], [lens[i] for i in some])
+
+
+def test_decode_fp8_many_kv_heads():
+    """More KV heads than resident blocks: one token group."""
+    import blackwell_b200 as bw
+    lens = [70, 3]
+    q, codes, sc, bt = make(lens, 700, 1, 64, 8, 95)
+    o, lse = run(q, codes, sc, bt, lens)
+    assert bw.stream_status() == 0
+    check(o, lse, q, codes, sc, bt, lens)
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_decode_fp8_random_shapes(seed):
+    import blackwell_b200 as bw
+    rng = np.random.default_rng(1000 + seed)
+    D, ps = int(rng.choice([64, 128])), int(rng.choice([8, 16, 32, 64, 128, 192]))
+    Hkv, G, B = int(rng.integers(1, 10)), int(rng.integers(1, 17)), int(rng.integers(1, 9))
+    lens = [int(n) for n in np.exp(rng.uniform(0, math.log(5000), B)).astype(int) - 1]
+    q, codes, sc, bt = make(lens, Hkv, G, D, ps, 2000 + seed)
+    o, lse = run(q, codes, sc, bt, lens)
+    assert bw.stream_status() == 0
+    check(o, lse, q, codes, sc, bt, lens)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_decode_fp8_wait_that_runs_out_is_reported(D):
+    """The K producers withhold their first tile (test hook): the consumers' bounded
+    waits expire, every block unwinds, the call reports BW_ERR_TIMEOUT, and the next
+    call on the stream is right."""
+    import blackwell_b200 as bw
+    from blackwell_b200 import _ffi
+    lens = [3000, 0, 700]
+    q, codes, sc, bt = make(lens, 4, 4, D, 16, 101)
+    old = bw.get_option(_ffi.BW_OPT_TIMEOUT_NS)
+    try:
+        bw.set_option(_ffi.BW_OPT_TIMEOUT_NS, 20_000_000)   # 20 ms
+        bw.set_option(_ffi.BW_OPT_DEBUG_FLAGS, 1)
+        run(q, codes, sc, bt, lens)
+        assert bw.stream_status() == _ffi.BW_ERR_TIMEOUT
+    finally:
+        bw.set_option(_ffi.BW_OPT_DEBUG_FLAGS, 0)
+        bw.set_option(_ffi.BW_OPT_TIMEOUT_NS, old)
+    o, lse = run(q, codes, sc, bt, lens)
+    assert bw.stream_status() == 0
+    check(o, lse, q, codes, sc, bt, lens)
