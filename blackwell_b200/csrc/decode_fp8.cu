@@ -476,8 +476,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
       }
     }
 
-    // ---- merge the four warps: references and sums of every head, then the
-    // outputs through the last stage (4 warps x 8 heads x D floats = its codes)
+    // ---- merge the warps: references and sums of every head, and the outputs,
+    // through shared memory; the outputs through the last stage, [warp][NT * 8
+    // heads][D] floats, columns permuted by 8 (h / 2 mod 4) so that the four lanes
+    // of a g do not meet in a bank.
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -490,70 +492,81 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
         ll += __shfl_xor_sync(0xffffffffu, ll, 4);
         ll += __shfl_xor_sync(0xffffffffu, ll, 8);
         ll += __shfl_xor_sync(0xffffffffu, ll, 16);
-        if (g == 0) {
+        m[nt][j] = mm;
+        l[nt][j] = ll;
+      }
+    float* part_o = reinterpret_cast<float*>(smem + s * C::kStage);
+    static_assert(kWarps * NT * 8 * D * 4 <= C::kStage, "the outputs fit a stage");
+    consumer_sync();   // the stage's codes, and the previous segment's sums, have been read
+    if (g == 0)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
           const int h = warp * 16 + nt * 8 + 2 * q4 + j;
-          red_m[h] = mm;
-          red_l[h] = ll;
+          red_m[h] = m[nt][j];
+          red_l[h] = l[nt][j];
           red_M[h] = M[nt][j];
         }
-      }
-    const bool whole = sg.tok0 == 0 && sg.tok1 == sg.len;
-    const int64_t part = (int64_t)(grp + sg.b) * p.Hkv + kvh;
-    float* part_o = reinterpret_cast<float*>(smem + s * C::kStage);   // [warp][8][D]
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      consumer_sync();   // the stage's codes (or the previous heads' outputs) have been read
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < D / 16; ++c)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-          *reinterpret_cast<float2*>(part_o + (warp * 8 + 2 * q4 + j) * D + 16 * c + 2 * g) =
+          *reinterpret_cast<float2*>(part_o + ((warp * NT + nt) * 8 + 2 * q4 + j) * D + ((16 * c + 2 * g) ^ (8 * q4))) =
               make_float2(o[nt][c][j], o[nt][c][2 + j]);
-      consumer_sync();
-      for (int i = tid; i < 8 * D / 4; i += kWarps * 32) {
-        const int hl = i / (D / 4), d = (i - hl * (D / 4)) * 4, h = nt * 8 + hl;
-        if (h >= p.G) break;
-        float mx = -INFINITY, Mx = -INFINITY;
+    if (tid == 0) bars.stop = *wc.abort_flag;
+    consumer_sync();
+    constexpr int kPer = kWarps * 32 / (NT * 8);   // threads a head
+    const int h = tid / kPer;
+    if (h < p.G) {
+      const bool whole = sg.tok0 == 0 && sg.tok1 == sg.len;
+      const int64_t part = ((int64_t)(grp + sg.b) * p.Hkv + kvh) * p.G + h;
+      const int64_t row = (int64_t)sg.b * p.Hq + kvh * p.G + h;
+      float mx = -INFINITY, Mx = -INFINITY, sum = 0.f, f[kWarps];
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          mx = fmaxf(mx, red_m[w * 16 + h]);
-          Mx = fmaxf(Mx, red_M[w * 16 + h]);
-        }
-        float sum = 0.f;
+      for (int w = 0; w < kWarps; ++w) {
+        mx = fmaxf(mx, red_m[w * 16 + h]);
+        Mx = fmaxf(Mx, red_M[w * 16 + h]);
+      }
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float mw = red_m[w * 16 + h], Mw = red_M[w * 16 + h];
+        sum += red_l[w * 16 + h] * (mw == -INFINITY ? 1.f : ex2f(mw - mx));
+        f[w] = Mw == -INFINITY ? 1.f : ex2f(Mw - Mx);
+      }
+      // o = a 2^Mx / (sum 2^mx); both powers may be far out, their quotient is the values' scale
+      const float to = (Mx == -INFINITY ? 1.f : ex2f(Mx - mx)) / sum;
+#pragma unroll
+      for (int d = (tid % kPer) * 4; d < D; d += kPer * 4) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float mw = red_m[w * 16 + h], Mw = red_M[w * 16 + h];
-          sum += red_l[w * 16 + h] * (mw == -INFINITY ? 1.f : ex2f(mw - mx));
-          const float f = Mw == -INFINITY ? 1.f : ex2f(Mw - Mx);
-          const float4 v = *reinterpret_cast<const float4*>(part_o + (w * 8 + hl) * D + d);
-          a.x = fmaf(f, v.x, a.x);
-          a.y = fmaf(f, v.y, a.y);
-          a.z = fmaf(f, v.z, a.z);
-          a.w = fmaf(f, v.w, a.w);
+          const float4 v = *reinterpret_cast<const float4*>(part_o + (w * NT * 8 + h) * D + (d ^ (8 * ((h >> 1) & 3))));
+          a.x = fmaf(f[w], v.x, a.x);
+          a.y = fmaf(f[w], v.y, a.y);
+          a.z = fmaf(f[w], v.z, a.z);
+          a.w = fmaf(f[w], v.w, a.w);
         }
-        // o = a 2^Mx / (sum 2^mx); both powers may be far out, their quotient is the values' scale
-        const float f = (Mx == -INFINITY ? 1.f : ex2f(Mx - mx)) / sum;
-        a.x *= f; a.y *= f; a.z *= f; a.w *= f;
-        const int64_t row = (int64_t)sg.b * p.Hq + kvh * p.G + h;
+        a.x *= to; a.y *= to; a.z *= to; a.w *= to;
         if (whole)
           *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.O) + row * D + d) =
               make_uint2(f32_to_bf16x2(a.x, a.y), f32_to_bf16x2(a.z, a.w));
         else
-          *reinterpret_cast<float4*>(p.o_part + (part * p.G + h) * D + d) = a;
-        if (d == 0) {
-          const float lse = (mx + __log2f(sum)) * 0.69314718055994531f;
-          if (!whole) p.lse_part[part * p.G + h] = lse;
-          else if (p.LSE) p.LSE[row] = lse;
-        }
+          *reinterpret_cast<float4*>(p.o_part + part * D + d) = a;
+      }
+      if (tid % kPer == 0) {
+        const float lse = (mx + __log2f(sum)) * 0.69314718055994531f;
+        if (!whole) p.lse_part[part] = lse;
+        else if (p.LSE) p.LSE[row] = lse;
       }
     }
-    // After a wait that ran out all four warps stop at the same segment, so that
-    // none waits at a barrier for one that has left.
-    if (tid == 0) bars.stop = *wc.abort_flag;
+    // After a wait that ran out all warps stop at the same segment, so that none
+    // waits at a barrier for one that has left, and no stage is given back any more.
+    if (*(volatile int*)&bars.stop) break;
     fence_proxy_async_smem();   // the stage goes back to the copies
-    consumer_sync();
-    if (*(volatile int*)&bars.stop) break;   // and no stage is given back any more
+    __syncwarp();
     if (lane == 0) mbar_arrive(&bars.empty[s]);
   }
 }
