@@ -312,7 +312,7 @@ int bw_gqa_decode_paged_fp8(const void* Q, const void* K_cache, const void* V_ca
   for (int i = 3; i < 31; ++i)
     if (page_size == 1 << i) p.page_shift = i;
   p.scale_log2 = scale * 1.4426950408889634f;
-  const int blocks = bw::decode_fp8_blocks(dev.num_sms, D, G);
+  const int blocks = bw::decode_fp8_blocks(dev.num_sms);
   p.groups = decode_groups(Hkv, blocks < kMaxDecodeBlocks ? blocks : kMaxDecodeBlocks);
   bw::Fp8DecodeMaps maps;
   const int64_t rows = (int64_t)num_pages * page_size;

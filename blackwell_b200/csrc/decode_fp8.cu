@@ -5,13 +5,34 @@
 //   o = sum_t p_t 2^ev_t v_t / sum_t p_t,  LSE = max x + ln sum_t p_t
 // with k_t, v_t the codes of token t.
 //
-// Split: the tiles of all sequences, one after the other, are dealt
-// to `groups` token groups in equal contiguous runs, so the load is even
-// whatever the lengths are; a group has one block per KV head (the heads of a
-// token are neighbours in memory and are read at the same time).  A run meets
-// a sequence in one segment.  A segment that holds the whole sequence writes
-// the result itself; the others leave (O, LSE) partials that the join kernel
-// merges in segment order, so results do not depend on timing.
+// Split: the tiles of all sequences, one after the other, are dealt to `groups`
+// token groups in equal contiguous runs, so the load is even whatever the
+// lengths are; a group has one block per KV head (the heads of a token are
+// neighbours in memory and are read at the same time).  A run meets a sequence
+// in one segment.  A segment that holds the whole sequence writes the result
+// itself; the others leave (O, LSE) partials that the join kernel merges in
+// segment order, so results do not depend on timing.  Runs are of whole tiles:
+// finer ones balance better but cut short sequences in two, and a segment costs
+// about 2 us (16 ragged sequences, heads of 64: 11 us against 12.5 with runs of
+// 64 tokens).
+//
+// 2 G flops a byte: bound by HBM.  The products take 13 to 18 % of the tensor
+// pipe through mma.sync; a tcgen05 product would want the f16 operands in shared
+// memory, where the codes are not, and 128 rows.  What had to be kept small
+// beside them is the work per code: the conversions (two codes an instruction,
+// no repacking) and the softmax, and the copies a page needs.
+//
+// Measured on B200 (device time; share of the 6.45 TB/s that a copy reaches):
+//   64 sequences of 1024 to 32768 tokens, 8 KV heads, G = 8, D = 128
+//     pages of 64   326 - 337 us   102 - 106 %   (bf16 cache: 2.2 times that)
+//     pages of 16   335 us         103 %
+//     pages of 8    390 us          88 %         one tensor copy per 8 rows
+//     D = 64        179 us          97 %
+//   32 sequences of 1000 to 32768, 4 KV heads, G = 16: 103 us, 84 %: two products
+//     and softmaxes a code, 8 consumer warps an SM hide their latency no further
+//   1 sequence of 131072: 49 us, 85 %: start, last merge and join take 7
+//   1 sequence of 517: 7.3 us: launch 0.4, tile counts 1, page index and first tile
+//     2.1, products 0.8, merge 0.9, join 2
 #include <cuda_bf16.h>
 
 #include <atomic>
@@ -35,9 +56,10 @@ constexpr int kMaxB = 4096;
 constexpr uint64_t kDrainNs = 20000000;   // 20 ms, thousands of times what a copy takes
 constexpr int kWarps = 4;      // consumers; one producer warp more for K and one for V
 constexpr int kThreads = 32 * (kWarps + 2);
-// Resident blocks an SM: registers (96 accumulators and Q fragments a thread in
-// the largest variant) and shared memory (about 67 KB a block).
-constexpr int blocks_per_sm(int D, int NT) { return 2; }
+// Resident blocks an SM: 97 KB of stages and up to 168 registers a thread each.
+// Three blocks of smaller tiles were slower (337 -> 349 us at the first shape
+// above), four too (355).
+constexpr int kBlocksPerSm = 2;
 
 // Tokens of sequence b: kv_lens[b], at least 0 and at most what its row of the
 // block table can hold.
@@ -82,7 +104,7 @@ template <int D>
 struct Cfg {
   static constexpr int kTile = tile_tokens(D);
   static constexpr int kHalf = kTile * D;            // K (or V) codes of a stage
-  static constexpr int kStage = 2 * kHalf;           // 16 KB
+  static constexpr int kStage = 2 * kHalf;           // 32 KB
   static constexpr int kStages = 3;
   static constexpr int kScales = kStages * kStage;
   static constexpr int kRed = kScales + kStages * 2 * kTile;    // m, l, M of 4 warps x 16 heads
@@ -163,7 +185,7 @@ __device__ __forceinline__ Segment next_segment(const Fp8DecodeParams& p, const 
   return s;
 }
 
-// One producer warp streams the tiles of the block's run through a ring of
+// Two producer warps stream the tiles of the block's run through a ring of
 // stages; four consumer warps take 16 tokens of every step each, keep their own
 // running softmax and output, and merge at the end of a segment.
 //
@@ -185,7 +207,7 @@ __device__ __forceinline__ Segment next_segment(const Fp8DecodeParams& p, const 
 // element.  Both references follow their maximum only when it has moved by more
 // than 2^8; m is per thread, M per warp (votes; shuffles only when it moves).
 template <int D, int NT>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     decode_fp8_kernel(const Fp8DecodeParams p, const __grid_constant__ Fp8DecodeMaps maps) {
   using C = Cfg<D>;
   constexpr int U = tile_steps(D), kTile = C::kTile;
@@ -300,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT))
   uint32_t n = 0;
   while (t0 < t1) {
     const Segment sg = next_segment<kTile>(p, prefix, t0, t1);
-    // Q of head (n tile) + g as f16, brought to [1, 2) by a power of two; columns in the codes' order
+    // Q of head 8 nt + g as f16, brought to [1, 2) by a power of two; columns in the codes' order
     uint32_t qb[NT][D / 16][2];
     float qs[NT][2];
 #pragma unroll
@@ -774,7 +796,7 @@ cudaError_t launch(const Fp8DecodeParams& p, const Fp8DecodeMaps& maps, cudaStre
 
 }  // namespace
 
-int decode_fp8_blocks(int num_sms, int D, int G) { return num_sms * blocks_per_sm(D, G <= 8 ? 1 : 2); }
+int decode_fp8_blocks(int num_sms) { return num_sms * kBlocksPerSm; }
 
 cudaError_t launch_decode_fp8(const Fp8DecodeParams& p, const Fp8DecodeMaps& maps, cudaStream_t stream) {
   if (p.D == 128) return p.G <= 8 ? launch<128, 1>(p, maps, stream) : launch<128, 2>(p, maps, stream);

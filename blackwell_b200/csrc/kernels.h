@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include "../../include/bw_attn.h"
+#include "fast_div.h"
 
 namespace bw {
 
@@ -167,7 +168,8 @@ struct RopeParams {
   int64_t table_len;
   const int* positions;      // [B, S] or null (position = s)
   int pos_offset;
-  int q_groups;              // set by the launch
+  int q_groups, block_tokens;   // set by the launch, like the divisions by units and S
+  FastDiv by_units, by_s;
 };
 cudaError_t launch_rope(const RopeParams& p, cudaStream_t stream);
 
@@ -187,6 +189,7 @@ struct KvWriteParams {
   int R, half;
   const int* positions;      // [T]
   int* err;
+  FastDiv by_heads, by_page;   // set by the launch: divisions by Hkv and page_size
 };
 cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream);
 
@@ -202,8 +205,9 @@ struct KvReadParams {
   int B, Hkv, D, page_size, num_pages, max_pages;
   int fp8;
   int* err;
+  FastDiv by_units, by_page;   // set by the launch: divisions by a token's units and page_size
 };
-cudaError_t launch_kv_read(const KvReadParams& p, int num_sms, cudaStream_t stream);
+cudaError_t launch_kv_read(KvReadParams p, int num_sms, cudaStream_t stream);
 
 // Decode over the paged 8-bit cache (decode_fp8.cu).
 struct Fp8DecodeParams {
@@ -232,7 +236,7 @@ struct Fp8DecodeMaps {
   CUtensorMap k, v;
 };
 // Blocks of the decode on a device of num_sms SMs (a full wave).
-int decode_fp8_blocks(int num_sms, int D, int G);
+int decode_fp8_blocks(int num_sms);
 cudaError_t launch_decode_fp8(const Fp8DecodeParams& p, const Fp8DecodeMaps& maps, cudaStream_t stream);
 
 // 2-D byte map with a box of (128 or 64 swizzled bytes, rows) (api.cu).

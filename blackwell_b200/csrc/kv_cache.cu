@@ -31,10 +31,10 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvWriteParams 
   const int sub = threadIdx.x % LPR;
   bool live = row < rows;
   if (!live) row = 0;   // stays for the warp's shuffles
-  const int64_t th = row >> 1;
+  const uint32_t th = (uint32_t)(row >> 1);   // T * Hkv is below 2^31
   const int is_v = (int)(row & 1);
-  const int64_t t = th / p.Hkv;
-  const int h = (int)(th - t * p.Hkv);
+  const int64_t t = p.by_heads.div(th);
+  const int h = (int)(th - (uint32_t)t * p.Hkv);
   const int64_t slot = p.slots[t];
   if (slot < 0) {
     live = false;   // padding
@@ -104,9 +104,8 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvWriteParams 
       *reinterpret_cast<uint2*>(out + e0) = lo;
       *reinterpret_cast<uint2*>(out + e1) = hi;
       if (sub == 0) {
-        const int64_t page = slot / p.page_size;
-        const int place = (int)(slot - page * p.page_size);
-        p.scales[((page * p.Hkv + h) * 2 + is_v) * p.page_size + place] = (uint8_t)(e + 127);
+        const uint32_t page = p.by_page.div((uint32_t)slot), place = (uint32_t)slot - page * p.page_size;
+        p.scales[(((int64_t)page * p.Hkv + h) * 2 + is_v) * p.page_size + place] = (uint8_t)(e + 127);
       }
     }
   }
@@ -145,9 +144,9 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvReadParams p)
         const uint32_t i = i0 + u * kThreads;
         dst[u] = -1;
         if (i >= n) continue;
-        const uint32_t tok = i / upr, unit = i - tok * upr;
+        const uint32_t tok = p.by_units.div(i), unit = i - tok * upr;
         const uint32_t at = (uint32_t)start + tok0 + tok;
-        const uint32_t pi = at / (uint32_t)p.page_size, place = at - pi * p.page_size;
+        const uint32_t pi = p.by_page.div(at), place = at - pi * p.page_size;
         const int page = bt[pi];
         if ((unsigned)page >= (unsigned)p.num_pages) {
           atomicCAS(p.err, 0, kErrIndexBit);
@@ -189,7 +188,9 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvReadParams p)
 }
 
 template <int D, bool FP8>
-cudaError_t write_launch(const KvWriteParams& p, cudaStream_t stream) {
+cudaError_t write_launch(KvWriteParams p, cudaStream_t stream) {
+  p.by_heads = FastDiv(p.Hkv);
+  p.by_page = FastDiv(p.page_size);
   const int64_t threads = (int64_t)p.T * p.Hkv * 2 * (D / 16);
   const dim3 blocks((unsigned)((threads + kThreads - 1) / kThreads));
   auto kern = p.table == nullptr ? kv_write_kernel<D, FP8, false, false>
@@ -205,7 +206,9 @@ cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream) {
   return p.fp8 ? write_launch<64, true>(p, stream) : write_launch<64, false>(p, stream);
 }
 
-cudaError_t launch_kv_read(const KvReadParams& p, int num_sms, cudaStream_t stream) {
+cudaError_t launch_kv_read(KvReadParams p, int num_sms, cudaStream_t stream) {
+  p.by_units = FastDiv((uint32_t)p.Hkv * (p.D / 8));
+  p.by_page = FastDiv(p.page_size);
   // Blocks for the longest span that the table's width or the output's rows
   // allow, at most about 16 an SM over all sequences.
   int64_t most = (int64_t)p.max_pages * p.page_size;

@@ -26,16 +26,22 @@ namespace {
 // quarter turn, goes to fp32.  Adding 1.5 * 2^52 rounds to a whole number whose
 // low bits are the quadrant, which saves the conversions between fp64 and
 // integers.  Bound by the stores.
-__global__ void rope_table_kernel(const RopeTableParams p) {
+constexpr int kTableThreads = 256, kTableBlocks = 6;   // resident blocks an SM, by registers
+
+__global__ void __launch_bounds__(kTableThreads, kTableBlocks) rope_table_kernel(const RopeTableParams p) {
   constexpr double kRound = 6755399441055744.0;   // 1.5 * 2^52
   const int i = threadIdx.x;
   const int half = p.R >> 1;
   const double f = 4.0 * p.turns[i];
   after_previous_kernel();
-  int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  const int64_t r0 = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
-  double pos = (double)(p.first + r);
-  for (; r < p.length; r += step, pos += (double)step) {
+  if (r0 >= p.length) return;
+  double pos = (double)(p.first + r0);
+  const double pos_step = (double)step;
+  float* out = p.table + r0 * p.R + i;
+  const int64_t out_step = step * p.R;
+  for (int64_t n = (p.length - r0 - 1) / step + 1; n > 0; --n, pos += pos_step, out += out_step) {
     const double quarters = f * pos;
     const double whole = quarters + kRound;
     const float x = (float)((quarters - (whole - kRound)) * 1.5707963267948966);   // |x| <= pi / 4
@@ -44,13 +50,11 @@ __global__ void rope_table_kernel(const RopeTableParams p) {
     const float s = fmaf(x * x2, fmaf(x2, fmaf(x2, fmaf(x2, 1.f / 362880.f, -1.f / 5040.f), 1.f / 120.f), -1.f / 6.f), x);
     const float c = fmaf(
         x2, fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, -1.f / 3628800.f, 1.f / 40320.f), -1.f / 720.f), 1.f / 24.f), -0.5f), 1.f);
-    const int q = __double2loint(whole) & 3;
-    float cc = (q & 1) ? s : c, ss = (q & 1) ? c : s;   // turn by q quarters
-    if (q == 1 || q == 2) cc = -cc;
-    if (q >= 2) ss = -ss;
-    float* row = p.table + r * p.R;
-    row[i] = cc * p.magnitude;
-    row[half + i] = ss * p.magnitude;
+    // turned by q quarters: (c, s), (-s, c), (-c, -s), (s, -c)
+    const uint32_t q = (uint32_t)__double2loint(whole);
+    const float cc = (q & 1) ? s : c, ss = (q & 1) ? c : s;
+    out[0] = __uint_as_float(__float_as_uint(cc * p.magnitude) ^ (((q + 1) & 2) << 30));
+    out[half] = __uint_as_float(__float_as_uint(ss * p.magnitude) ^ ((q & 2) << 30));
   }
 }
 
@@ -83,11 +87,11 @@ template <typename T, bool HALF, int kHeads>
 __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
   constexpr int V = Vec<T>::V;
   after_previous_kernel();
-  const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t tok = idx / p.units;
-  if (tok >= (int64_t)p.B * p.S) return;
-  const int unit = (int)(idx - tok * p.units);
-  const int b = (int)(tok / p.S), s = (int)(tok - (int64_t)b * p.S);
+  const uint32_t in_block = p.by_units.div(threadIdx.x);   // token of the block
+  const int64_t tok = (int64_t)blockIdx.x * p.block_tokens + in_block;
+  if (in_block >= (uint32_t)p.block_tokens || tok >= (int64_t)p.B * p.S) return;
+  const int unit = (int)(threadIdx.x - in_block * p.units);
+  const int b = (int)p.by_s.div((uint32_t)tok), s = (int)tok - b * p.S;
   const bool is_k = (int)blockIdx.y >= p.q_groups;
   const RopeTensor& t = is_k ? p.k : p.q;
   const int h0 = ((int)blockIdx.y - (is_k ? p.q_groups : 0)) * kHeads;
@@ -145,7 +149,11 @@ cudaError_t launch(RopeParams p, cudaStream_t stream) {
   const int64_t threads = (int64_t)p.B * p.S * p.units;
   // Few tokens: small blocks, so that the work spreads over the SMs.
   const int block = threads <= 148 * 64 ? 64 : 256;
-  const dim3 grid((unsigned)((threads + block - 1) / block), (unsigned)(p.q_groups + k_groups));
+  p.block_tokens = block / p.units;   // units: at most 64
+  p.by_units = FastDiv(p.units);
+  p.by_s = FastDiv(p.S);
+  const int64_t tokens = (int64_t)p.B * p.S;
+  const dim3 grid((unsigned)((tokens + p.block_tokens - 1) / p.block_tokens), (unsigned)(p.q_groups + k_groups));
   return launch_early(p.half ? rope_kernel<T, true, kHeads> : rope_kernel<T, false, kHeads>, grid, dim3(block), 0,
                       stream, p);
 }
@@ -154,9 +162,9 @@ cudaError_t launch(RopeParams p, cudaStream_t stream) {
 
 cudaError_t launch_rope_table(const RopeTableParams& p, int num_sms, cudaStream_t stream) {
   const int half = p.R / 2;
-  const dim3 block((unsigned)half, (unsigned)(half >= 256 ? 1 : 256 / half));
+  const dim3 block((unsigned)half, (unsigned)(kTableThreads / half));   // half: at most 256
   int64_t blocks = (p.length + block.y - 1) / block.y;
-  const int64_t cap = (int64_t)num_sms * 8;
+  const int64_t cap = (int64_t)num_sms * kTableBlocks;
   if (blocks > cap) blocks = cap;
   return launch_early(rope_table_kernel, dim3((unsigned)blocks), block, 0, stream, p);
 }

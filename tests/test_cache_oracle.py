@@ -70,18 +70,20 @@ def test_table_matches_plain_formula():
             assert abs(t[p - 5, i] - math.cos(a)) < 1e-14 and abs(t[p - 5, 8 + i] - math.sin(a)) < 1e-14
 
 
-@pytest.mark.parametrize("Hkv,blocks", [(1, 592), (8, 592), (12, 444), (16, 1024), (700, 592)])
-def test_decode_split_covers_every_tile_once(Hkv, blocks):
-    """Segments of the decode (decode_fp8.cu: equal runs of 64-token tiles): every
-    tile belongs to one segment, a segment's partial index (group + sequence) is
-    its own and within (groups + B), and the join's range of groups is the segments'."""
+@pytest.mark.parametrize("tile", [128, 256])
+@pytest.mark.parametrize("Hkv,blocks", [(1, 296), (8, 296), (12, 444), (16, 1024), (700, 296)])
+def test_decode_split_covers_every_tile_once(Hkv, blocks, tile):
+    """Segments of the decode (decode_fp8.cu: equal runs of tiles, whole tiles of a
+    sequence): every tile belongs to one segment, a segment's partial index (group +
+    sequence) is its own and within (groups + B), and the join's range of groups is
+    the segments'."""
     rng = np.random.default_rng(Hkv)
     groups = max(blocks // Hkv, 1)
     for lens in ([0], [1], [517], [64, 0, 65, 0, 0, 4096], list(rng.integers(0, 9000, 70)), [131072], [0, 0]):
-        tiles = [(n + 63) // 64 for n in lens]
+        tiles = [(n + tile - 1) // tile for n in lens]
         prefix = np.concatenate([[0], np.cumsum(tiles)]).astype(int)
         total = prefix[-1]
-        per = max((total + groups - 1) // groups, 4)
+        per = max((total + groups - 1) // groups, 1)
         seen, parts, by_seq = set(), set(), {}
         for g in range(groups):
             t0, t1 = min(g * per, total), min(g * per + per, total)
