@@ -13,7 +13,6 @@ The 8-bit cache is ``k_cache`` / ``v_cache`` float8_e4m3fn
 """
 from __future__ import annotations
 
-import ctypes
 import importlib
 import math
 
@@ -52,9 +51,8 @@ def rope_table(length, rotary_dim, base=10000.0, scaling="none", factor=1.0, ori
                           device=torch.device("cuda", torch.cuda.current_device()))
     elif out.shape != (length, rotary_dim):
         raise ValueError(f"out must be [{length}, {rotary_dim}], got {tuple(out.shape)}")
-    s = _ffi.BwRopeScaling(_SCALINGS[scaling], base, factor, original_length, attention_factor, beta_fast, beta_slow,
-                           low_freq_factor, high_freq_factor)
-    rc = (_front or _load()).rope_table(out, first, ctypes.addressof(s))
+    rc = (_front or _load()).rope_table(out, first, _SCALINGS[scaling], base, factor, original_length, attention_factor,
+                                        beta_fast, beta_slow, low_freq_factor, high_freq_factor)
     if rc:
         _ffi.check(rc, "bw_rope_table")
     return out

@@ -24,7 +24,7 @@
 //
 // Measured on B200 (device time; share of the 6.45 TB/s that a copy reaches):
 //   64 sequences of 1024 to 32768 tokens, 8 KV heads, G = 8, D = 128
-//     pages of 64   326 - 337 us   102 - 106 %   (bf16 cache: 2.2 times that)
+//     pages of 64   326 - 356 us   97 - 106 %   (by box; the bf16 cache has twice the bytes)
 //     pages of 16   335 us         103 %
 //     pages of 8    390 us          88 %         one tensor copy per 8 rows
 //     D = 64        179 us          97 %

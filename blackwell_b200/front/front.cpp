@@ -100,14 +100,22 @@ int small(const char* name, int64_t v) {
 
 // ------------------------------------------------------------------ the functions
 
-// rope_table(out, first, scaling address)
+double real(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw Refused{};
+  return v;
+}
+
+// rope_table(out, first, kind, and the eight numbers of bw_rope_scaling in their order)
 int rope_table(PyObject* const* a) {
   const Tensor* out = tensor(a[0], "out");
   if (out->dim() != 2) refuse(PyExc_ValueError, "out must be [length, rotary_dim]");
   want("out", *out, at::kFloat, {out->size(0), out->size(1)});
+  bw_rope_scaling s{int32(a[2], "kind"), real(a[3]), real(a[4]), real(a[5]), real(a[6]), real(a[7]), real(a[8]), real(a[9]),
+                    real(a[10])};
   void* stream = stream_for({out});
-  const auto* s = reinterpret_cast<const bw_rope_scaling*>(PyLong_AsVoidPtr(a[2]));
-  return bw_rope_table(static_cast<float*>(ptr(out)), out->size(0), small("rotary_dim", out->size(1)), integer(a[1]), s, stream);
+  return bw_rope_table(static_cast<float*>(ptr(out)), out->size(0), small("rotary_dim", out->size(1)), integer(a[1]), &s,
+                       stream);
 }
 
 // Strides of the (b, h, s) axes of a [B, H, S, D] tensor; of [tokens, H, D]: B =
@@ -260,8 +268,7 @@ int gqa_decode_paged_fp8(PyObject* const* a) {
   want("out", *out, at::kBFloat16, {B, Hq, c.D});
   want("lse", *lse, at::kFloat, {B, Hq});
   if (!ws->is_contiguous()) refuse(PyExc_ValueError, "workspace must be contiguous");
-  const double scale = PyFloat_AsDouble(a[6]);
-  if (scale == -1.0 && PyErr_Occurred()) throw Refused{};
+  const double scale = real(a[6]);
   void* stream = stream_for({q, kc, vc, scales, bt, lens, ws, out, lse});
   return bw_gqa_decode_paged_fp8(ptr(q), ptr(kc), ptr(vc), static_cast<const uint8_t*>(ptr(scales)),
                                  static_cast<const int*>(ptr(bt)), static_cast<const int*>(ptr(lens)), ptr(out),
@@ -288,7 +295,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 #define BW_METHOD(f, n) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&call<f, n>)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {BW_METHOD(rope_table, 3), BW_METHOD(rope, 9), BW_METHOD(kv_cache_write, 9),
+PyMethodDef methods[] = {BW_METHOD(rope_table, 11), BW_METHOD(rope, 9), BW_METHOD(kv_cache_write, 9),
                          BW_METHOD(kv_cache_read, 9), BW_METHOD(gqa_decode_paged_fp8, 10), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_front", "Checked calls of the rotary and cache entry points.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
