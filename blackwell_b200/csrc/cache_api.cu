@@ -161,7 +161,7 @@ int bw_rope(const void* Q, void* Q_out, const void* K, void* K_out, int dtype, i
   bw::DeviceInfo dev;
   rc = bw::device_info(stream, &dev);
   if (rc != BW_OK) return rc;
-  return bw::launch_rope(p, static_cast<cudaStream_t>(stream)) == cudaSuccess ? BW_OK : BW_ERR_CUDA;
+  return bw::launch_rope(p, dev.num_sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? BW_OK : BW_ERR_CUDA;
 }
 
 int bw_kv_cache_write(const void* K, const void* V, const int64_t* k_strides, const int64_t* v_strides, int T, int Hkv,

@@ -171,7 +171,7 @@ struct RopeParams {
   int q_groups, block_tokens;   // set by the launch, like the divisions by units and S
   FastDiv by_units, by_s;
 };
-cudaError_t launch_rope(const RopeParams& p, cudaStream_t stream);
+cudaError_t launch_rope(const RopeParams& p, int num_sms, cudaStream_t stream);
 
 // Paged cache (kv_cache.cu): [num_pages, page_size, Hkv, D] bf16 or e4m3,
 // scales uint8 [num_pages, Hkv, 2, page_size] beside e4m3.

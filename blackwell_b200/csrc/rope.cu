@@ -78,13 +78,15 @@ struct Vec<float> {
   }
 };
 
+constexpr int kRopeThreads = 128, kRopeBlocks = 8;   // resident blocks an SM, at four heads a thread
+
 // A thread owns one unit of a token: two vectors of 16 bytes, R / 2 elements
 // apart, that rotate with each other (half layout) or each within itself, or two
 // vectors behind the rotary part; neighbouring threads read neighbouring
 // vectors.  It reads its cos and sin once and applies them to kHeads heads, whose
 // loads are all in flight together.
 template <typename T, bool HALF, int kHeads>
-__global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) {
   constexpr int V = Vec<T>::V;
   after_previous_kernel();
   const uint32_t in_block = p.by_units.div(threadIdx.x);   // token of the block
@@ -143,19 +145,27 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
 }
 
 template <typename T, int kHeads>
-cudaError_t launch(RopeParams p, cudaStream_t stream) {
+cudaError_t launch(RopeParams p, unsigned token_blocks, cudaStream_t stream) {
   p.q_groups = (p.q.H + kHeads - 1) / kHeads;
   const int k_groups = (p.k.H + kHeads - 1) / kHeads;
-  const int64_t threads = (int64_t)p.B * p.S * p.units;
-  // Few tokens: small blocks, so that the work spreads over the SMs.
-  const int block = threads <= 148 * 64 ? 64 : 256;
-  p.block_tokens = block / p.units;   // units: at most 64
+  return launch_early(p.half ? rope_kernel<T, true, kHeads> : rope_kernel<T, false, kHeads>,
+                      dim3(token_blocks, (unsigned)(p.q_groups + k_groups)), dim3(kRopeThreads), 0, stream, p);
+}
+
+// Four heads a thread re-use its angles and keep eight loads in flight; where that
+// leaves less than a wave of blocks, two heads spread the work (2960 x 3 tokens, 8
+// heads of 80: 5.1 -> 4.8 us; 1777 x 3 tokens, 16 heads of 64 in fp32, more than a
+// wave: 8.8 us with four heads, 9.6 with two; 4 x 4096 tokens, 40 heads: 54.8, 55.3).
+template <typename T>
+cudaError_t launch_heads(RopeParams p, int num_sms, cudaStream_t stream) {
+  p.block_tokens = kRopeThreads / p.units;   // units: at most 64
   p.by_units = FastDiv(p.units);
   p.by_s = FastDiv(p.S);
   const int64_t tokens = (int64_t)p.B * p.S;
-  const dim3 grid((unsigned)((tokens + p.block_tokens - 1) / p.block_tokens), (unsigned)(p.q_groups + k_groups));
-  return launch_early(p.half ? rope_kernel<T, true, kHeads> : rope_kernel<T, false, kHeads>, grid, dim3(block), 0,
-                      stream, p);
+  const int64_t bx = (tokens + p.block_tokens - 1) / p.block_tokens;
+  const int64_t blocks = bx * ((p.q.H + 3) / 4 + (p.k.H + 3) / 4);
+  return blocks >= (int64_t)num_sms * kRopeBlocks ? launch<T, 4>(p, (unsigned)bx, stream)
+                                                  : launch<T, 2>(p, (unsigned)bx, stream);
 }
 
 }  // namespace
@@ -169,8 +179,8 @@ cudaError_t launch_rope_table(const RopeTableParams& p, int num_sms, cudaStream_
   return launch_early(rope_table_kernel, dim3((unsigned)blocks), block, 0, stream, p);
 }
 
-cudaError_t launch_rope(const RopeParams& p, cudaStream_t stream) {
-  return p.fp32 ? launch<float, 4>(p, stream) : launch<__nv_bfloat16, 4>(p, stream);
+cudaError_t launch_rope(const RopeParams& p, int num_sms, cudaStream_t stream) {
+  return p.fp32 ? launch_heads<float>(p, num_sms, stream) : launch_heads<__nv_bfloat16>(p, num_sms, stream);
 }
 
 }  // namespace bw
