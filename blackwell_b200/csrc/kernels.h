@@ -205,7 +205,8 @@ struct KvReadParams {
   int B, Hkv, D, page_size, num_pages, max_pages;
   int fp8;
   int* err;
-  FastDiv by_units, by_page;   // set by the launch: divisions by a token's units and page_size
+  int block_tokens;          // set by the launch, like the divisions by a token's units and page_size
+  FastDiv by_units, by_page;
 };
 cudaError_t launch_kv_read(KvReadParams p, int num_sms, cudaStream_t stream);
 
