@@ -167,6 +167,15 @@ __device__ __forceinline__ void arrive_after_copies(uint64_t* bar) {
 struct Segment {
   int b, len, tok0, tok1;   // tokens [tok0, tok1) of sequence b
 };
+// The first tile from t on with which a sequence begins (or the end of all).
+__device__ __forceinline__ int sequence_start(const int* prefix, int B, int t) {
+  int lo = 0, hi = B;   // the first b with prefix[b] >= t
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] < t) lo = mid + 1; else hi = mid;
+  }
+  return prefix[lo];
+}
 // The segment that begins at tile t0 of the run [t0, t1); t0 moves behind it.
 template <int kTile>
 __device__ __forceinline__ Segment next_segment(const Fp8DecodeParams& p, const int* prefix, int& t0, int t1) {
@@ -206,7 +215,9 @@ __device__ __forceinline__ Segment next_segment(const Fp8DecodeParams& p, const 
 // The denominator has its own reference m (the maximum of x): one more ex2 an
 // element.  Both references follow their maximum only when it has moved by more
 // than 2^8; m is per thread, M per warp (votes; shuffles only when it moves).
-template <int D, int NT>
+//
+// WHOLE: runs begin and end with a sequence, so that none is cut and no join follows.
+template <int D, int NT, bool WHOLE>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     decode_fp8_kernel(const Fp8DecodeParams p, const __grid_constant__ Fp8DecodeMaps maps) {
   using C = Cfg<D>;
@@ -233,8 +244,11 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   const int total = prefix[p.B], per = tiles_per_group(total, p.groups);
   if (blockIdx.x == 0)
     for (int b = tid; b <= p.B; b += kThreads) p.prefix[b] = prefix[b];
-  int t0 = min(grp * per, total);
-  const int t1 = min(t0 + per, total);
+  int t0 = min(grp * per, total), t1 = min(t0 + per, total);
+  if constexpr (WHOLE) {
+    t0 = sequence_start(prefix, p.B, t0);
+    t1 = sequence_start(prefix, p.B, t1);
+  }
   const WaitCtl wc{&bars.abort_flag, p.err, p.timeout_ns, 48 + warp};
   const uint32_t sbase = smem_u32(smem);
   const int bh = p.page_size < 64 ? p.page_size : 64;   // rows of a piece
@@ -319,6 +333,14 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   const uint32_t row_off = (uint32_t)lrow * D;   // pieces follow one another: a row's place does not depend on bh
   const uint32_t swz = D == 128 ? (lrow & 7) : ((lrow >> 1) & 3);
   const uint32_t chunk0 = lane >> 4;
+  if constexpr (WHOLE)   // the sequences without tokens are written here, not by the join
+    for (int b = grp; b < p.B; b += p.groups) {
+      if (prefix[b + 1] != prefix[b]) continue;
+      const int64_t row = (int64_t)b * p.Hq + kvh * p.G;
+      for (int i = tid; i < p.G * D / 8; i += kWarps * 32)
+        reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.O) + row * D)[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (p.LSE && tid < p.G) p.LSE[row + tid] = -INFINITY;
+    }
   uint32_t n = 0;
   while (t0 < t1) {
     const Segment sg = next_segment<kTile>(p, prefix, t0, t1);
@@ -763,10 +785,9 @@ __global__ void __launch_bounds__(128) decode_fp8_join_few_kernel(const Fp8Decod
   }
 }
 
-template <int D, int NT>
-cudaError_t launch(const Fp8DecodeParams& p, const Fp8DecodeMaps& maps, cudaStream_t stream) {
-  auto kern = decode_fp8_kernel<D, NT>;
-  const int bytes = Cfg<D>::kPrefix + (p.B + 1) * 4 + 1024;
+template <int D, int NT, bool WHOLE>
+cudaError_t launch_main(const Fp8DecodeParams& p, const Fp8DecodeMaps& maps, cudaStream_t stream) {
+  auto kern = decode_fp8_kernel<D, NT, WHOLE>;
   // Once per device; the limit, not what a launch takes, so it covers every B.
   static std::atomic<uint64_t> allowed{0};
   int dev = 0;
@@ -777,7 +798,20 @@ cudaError_t launch(const Fp8DecodeParams& p, const Fp8DecodeMaps& maps, cudaStre
     if (e != cudaSuccess) return e;
     if (dev < 64) allowed |= uint64_t(1) << dev;
   }
-  e = launch_early(kern, dim3(p.groups * p.Hkv), dim3(kThreads), bytes, stream, p, maps);
+  return launch_early(kern, dim3(p.groups * p.Hkv), dim3(kThreads), Cfg<D>::kPrefix + (p.B + 1) * 4 + 1024, stream, p, maps);
+}
+
+template <int D, int NT>
+cudaError_t launch(const Fp8DecodeParams& p, const Fp8DecodeMaps& maps, cudaStream_t stream) {
+  // Sequences of a few tiles (by the table's width) are not cut: the join and its
+  // launch would cost more than a block's further tiles.  Up to two tiles always
+  // (48 sequences of up to 107 tokens, 4 KV heads, D = 64: 8.0 -> 6.8 us), up to
+  // four where sequences and heads occupy the GPU (16 of up to 500 tokens, 8 KV
+  // heads: 10.8 -> 9.4; 2 of up to 1000, 2 KV heads, D = 64: 8.0 cut, 8.9 not).
+  // With up to eight it is slower or the same (16 of up to 1000: 12.0 cut, 13.5 not).
+  const int tiles = (p.max_tokens + Cfg<D>::kTile - 1) / Cfg<D>::kTile;
+  if (tiles <= 2 || (tiles <= 4 && 4 * p.B >= p.groups)) return launch_main<D, NT, true>(p, maps, stream);
+  const cudaError_t e = launch_main<D, NT, false>(p, maps, stream);
   if (e != cudaSuccess) return e;
   // A sequence has about groups / B segments, and no more than tiles.  Many (few KV
   // heads, few long sequences): wide blocks with 4 loads in flight a thread (131072

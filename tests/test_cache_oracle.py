@@ -101,3 +101,27 @@ def test_decode_split_covers_every_tile_once(Hkv, blocks, tile):
         assert len(seen) == total
         for b, gs in by_seq.items():
             assert gs == list(range(prefix[b] // per, (prefix[b + 1] - 1) // per + 1))
+
+
+@pytest.mark.parametrize("groups", [1, 4, 37, 74, 296])
+def test_decode_runs_of_whole_sequences(groups):
+    """Short tables: a run begins and ends with a sequence, so every sequence with
+    tokens is in exactly one run, whole."""
+    rng = np.random.default_rng(groups)
+    for tiles in ([1], [0], [2, 0, 1, 2, 2, 0], list(rng.integers(0, 5, 300)), [0, 0, 4], [4] * 40):
+        prefix = np.concatenate([[0], np.cumsum(tiles)]).astype(int)
+        total, B = prefix[-1], len(tiles)
+        per = max((total + groups - 1) // groups, 1)
+        start = lambda t: prefix[np.searchsorted(prefix, t)]   # noqa: E731
+        seen = []
+        for g in range(groups):
+            t0, t1 = start(min(g * per, total)), start(min(g * per + per, total))
+            while t0 < t1:
+                b = int(np.searchsorted(prefix[:-1], t0, side="right")) - 1
+                assert prefix[b] == t0 and prefix[b + 1] <= t1
+                seen.append(b)
+                t0 = prefix[b + 1]
+        assert seen == [b for b in range(B) if tiles[b]]
+        # the sequences without tokens, by groups
+        assert sorted(b for g in range(groups) for b in range(g, B, groups) if not tiles[b]) == \
+            [b for b in range(B) if not tiles[b]]

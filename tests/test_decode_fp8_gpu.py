@@ -294,3 +294,15 @@ def test_decode_fp8_wait_that_runs_out_is_reported(D):
     o, lse = run(q, codes, sc, bt, lens)
     assert bw.stream_status() == 0
     check(o, lse, q, codes, sc, bt, lens)
+
+
+@pytest.mark.parametrize("D,extra", [(64, 0), (64, 40), (128, 0), (128, 40)])
+def test_decode_fp8_tables_wide_and_narrow_agree(D, extra):
+    """The same sequences with a table of few pages (they are not cut then) and with a
+    wider one (cut and joined): both within the bounds, empty sequences among them."""
+    import blackwell_b200 as bw
+    lens = [0, 200, 17, 0, 128, 129, 1, 0]
+    q, codes, sc, bt = make(lens, 2, 4, D, 16, 111, width_extra=extra)
+    o, lse = run(q, codes, sc, bt, lens)
+    assert bw.stream_status() == 0
+    check(o, lse, q, codes, sc, bt, lens)
