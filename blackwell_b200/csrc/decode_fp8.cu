@@ -479,6 +479,37 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
         }
       }
       if (__any_sync(0xffffffffu, moved)) {
+        // A row of zeros (scale byte 127) adds nothing and must not raise M: the
+        // rows that carry the output would fall below f16.  Its y goes to -inf.
+        // Where M does not move its weight is at most 2^8 and its codes say the rest.
+        bool at_127 = false;
+#pragma unroll
+        for (int u = 0; u < N; ++u) at_127 |= ev[u][0] == 0.f || ev[u][1] == 0.f;
+        if (__any_sync(0xffffffffu, at_127)) {
+          uint32_t some_code = 0;   // bit 2 u + i: token 8 i + g of step u has a code other than 0 and NaN
+          const uint8_t* vrow = smem + s * C::kStage + C::kHalf + (u0 * kStep + warp * 16 + g) * D + q4 * (D / 4);
+#pragma unroll 1
+          for (int e = 0; e < 2 * N; ++e) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+              const uint4 w = reinterpret_cast<const uint4*>(vrow + ((e >> 1) * kStep + (e & 1) * 8) * D)[c];
+              // a byte's magnitude + 1 has a bit of 0x7e unless it was 0 or 0x7f
+              any |= ((w.x & 0x7f7f7f7fu) + 0x01010101u) | ((w.y & 0x7f7f7f7fu) + 0x01010101u) |
+                     ((w.z & 0x7f7f7f7fu) + 0x01010101u) | ((w.w & 0x7f7f7f7fu) + 0x01010101u);
+            }
+            some_code |= (any & 0x7e7e7e7eu) ? 1u << e : 0u;
+          }
+          some_code |= __shfl_xor_sync(0xffffffffu, some_code, 1);
+          some_code |= __shfl_xor_sync(0xffffffffu, some_code, 2);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int e = 0; e < 2 * N; ++e)
+                if (!(some_code >> e & 1)) y[nt][j][e] = -INFINITY;
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

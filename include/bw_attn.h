@@ -312,7 +312,8 @@ BW_API int bw_kv_cache_read(const void* K_cache, const void* V_cache, const uint
  * values enter at their exact values, products are of fp16 and summed in fp32: Q is
  * exact there down to 2^-14 of its row's largest element, and a token's weight
  * times its value scale is rounded to fp16 (2^-11 of itself, 2^-25 of the largest
- * one of the sequence's part below that).  O bf16, LSE natural log or NULL; a
+ * one of the sequence's part below that; a value row of zeros, which has the
+ * scale byte 127, is none of them).  O bf16, LSE natural log or NULL; a
  * sequence without tokens gives O = 0 and LSE = -inf.  O and LSE may not overlap
  * an input.  Codes, scales and table entries past kv_lens[b] are not used,
  * whatever they hold.  A length beyond the table is cut to it.  A page outside
