@@ -127,7 +127,8 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvReadParams p)
   if (len <= 0) return;
   const int64_t start = p.kv_starts ? p.kv_starts[b] : 0;
   const int64_t out0 = p.out_offsets[b];
-  if (start < 0 || start + len > (int64_t)p.max_pages * p.page_size || out0 < 0 || out0 + len > p.total_rows) {
+  // (out0 + len might pass 2^63)
+  if (start < 0 || start + len > (int64_t)p.max_pages * p.page_size || out0 < 0 || out0 > p.total_rows - len) {
     if (blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(p.err, 0, kErrIndexBit);
     return;
   }
