@@ -68,14 +68,20 @@ __device__ __forceinline__ int seq_len(const Fp8DecodeParams& p, int b) {
   return len < 0 ? 0 : min(len, p.max_tokens);
 }
 
-// prefix[b] = tiles before sequence b (prefix[B] = all), by the whole block.
+// prefix[b] = tiles before sequence b (prefix[B] = all), by the whole block.  Every
+// length is read once, so that the counts fit together whatever happens to
+// kv_lens meanwhile.
 template <int kTile>
 __device__ void tile_prefix(const Fp8DecodeParams& p, int* prefix, int* warp_sum) {
   const int tid = threadIdx.x, nth = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.B + nth - 1) / nth;
   const int b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
   int mine = 0;
-  for (int b = b0; b < b1; ++b) mine += (seq_len(p, b) + kTile - 1) / kTile;
+  for (int b = b0; b < b1; ++b) {
+    const int tiles = (seq_len(p, b) + kTile - 1) / kTile;
+    prefix[b] = tiles;
+    mine += tiles;
+  }
   int x = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -87,8 +93,9 @@ __device__ void tile_prefix(const Fp8DecodeParams& p, int* prefix, int* warp_sum
   int before = x - mine;
   for (int w = 0; w < warp; ++w) before += warp_sum[w];
   for (int b = b0; b < b1; ++b) {
+    const int tiles = prefix[b];
     prefix[b] = before;
-    before += (seq_len(p, b) + kTile - 1) / kTile;
+    before += tiles;
   }
   if (tid == nth - 1) prefix[p.B] = before;
   __syncthreads();
@@ -186,7 +193,11 @@ __device__ __forceinline__ Segment next_segment(const Fp8DecodeParams& p, const 
   }
   Segment s;
   s.b = lo;
-  s.len = seq_len(p, lo);
+  // The last tile decides the length; the tiles are the prefix's: a length that the
+  // caller has changed since (an error) must not lead to a segment without tokens,
+  // nor the warps of a block to different tiles.
+  const int tiles = prefix[lo + 1] - prefix[lo];
+  s.len = min(max(seq_len(p, lo), (tiles - 1) * kTile + 1), tiles * kTile);
   const int end = min(t1, prefix[lo + 1]);
   s.tok0 = (t0 - prefix[lo]) * kTile;
   s.tok1 = min((end - prefix[lo]) * kTile, s.len);
