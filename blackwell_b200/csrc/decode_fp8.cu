@@ -464,7 +464,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
             const int u = e / 2, i = e % 2;
             float a = acc[u][nt][0][2 * i + j];
             if constexpr (kChains == 2) a += acc[u][nt][1][2 * i + j];
-            x[j][e] = a * ks[u][i] * qs[nt][j];
+            // Key and query scales may be far out and make up for each other: a small qs goes to ks first, a large one last.
+            x[j][e] = a * (ks[u][i] * fminf(qs[nt][j], 1.f)) * fmaxf(qs[nt][j], 1.f);
           }
         if (some) {
 #pragma unroll
@@ -648,8 +649,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
         sum += red_l[w * 16 + h] * (mw == -INFINITY ? 1.f : ex2f(mw - mx));
         f[w] = Mw == -INFINITY ? 1.f : ex2f(Mw - Mx);
       }
-      // o = a 2^Mx / (sum 2^mx); both powers may be far out, their quotient is the values' scale
-      const float to = (Mx == -INFINITY ? 1.f : ex2f(Mx - mx)) / sum;
+      // o = a 2^Mx / (sum 2^mx); both powers may be far out, their quotient is the values' scale, and up to 2^8
+      // more (2^128 at the largest values) since mx lags: a part of a large one comes after the division.
+      const float back = Mx - mx > 64.f ? 65536.f : 1.f;
+      const float to = (Mx == -INFINITY ? 1.f : ex2f(Mx - mx - (back == 1.f ? 0.f : 16.f))) / sum;
 #pragma unroll
       for (int d = (tid % kPer) * 4; d < D; d += kPer * 4) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -662,6 +665,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
           a.w = fmaf(f[w], v.w, a.w);
         }
         a.x *= to; a.y *= to; a.z *= to; a.w *= to;
+        a.x *= back; a.y *= back; a.z *= back; a.w *= back;
         if (whole)
           *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.O) + row * D + d) =
               make_uint2(f32_to_bf16x2(a.x, a.y), f32_to_bf16x2(a.z, a.w));
@@ -682,6 +686,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     if (lane == 0) mbar_arrive(&bars.empty[s]);
   }
 }
+
+// The joins sum their segments times 2^-10: up to 2^10 of them (kMaxDecodeBlocks)
+// whose values are near fp32's largest have a mean in range and a sum beyond it.
+constexpr float kJoinDown = 1.f / 1024.f, kJoinUp = 1024.f;
 
 // One block of T threads per (sequence, query head): the segments of the sequence
 // are the groups whose runs meet its tiles; kUnroll times the segments that fit
@@ -733,12 +741,12 @@ __global__ void __launch_bounds__(T) decode_fp8_join_kernel(const Fp8DecodeParam
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
       if (i0 + u * kRows < n) {
-        const float e = __expf(w[u] - sub);
+        const float e = __expf(w[u] - sub), ed = e * kJoinDown;
         wsum += e;
-        acc.x = fmaf(e, v[u].x, acc.x);
-        acc.y = fmaf(e, v[u].y, acc.y);
-        acc.z = fmaf(e, v[u].z, acc.z);
-        acc.w = fmaf(e, v[u].w, acc.w);
+        acc.x = fmaf(ed, v[u].x, acc.x);
+        acc.y = fmaf(ed, v[u].y, acc.y);
+        acc.z = fmaf(ed, v[u].z, acc.z);
+        acc.w = fmaf(ed, v[u].w, acc.w);
       }
   }
   part[r][lane] = acc;
@@ -751,8 +759,8 @@ __global__ void __launch_bounds__(T) decode_fp8_join_kernel(const Fp8DecodeParam
       wsum += wsum_s[i];
     }
     const float inv = 1.f / wsum;
-    *reinterpret_cast<uint2*>(O + 4 * lane) =
-        make_uint2(f32_to_bf16x2(acc.x * inv, acc.y * inv), f32_to_bf16x2(acc.z * inv, acc.w * inv));
+    *reinterpret_cast<uint2*>(O + 4 * lane) = make_uint2(f32_to_bf16x2(acc.x * inv * kJoinUp, acc.y * inv * kJoinUp),
+                                                         f32_to_bf16x2(acc.z * inv * kJoinUp, acc.w * inv * kJoinUp));
     if (p.LSE && lane == 0) p.LSE[row] = sub + __logf(wsum);
   }
 }
@@ -804,11 +812,12 @@ __global__ void __launch_bounds__(128) decode_fp8_join_few_kernel(const Fp8Decod
         const int j = j0 + u * kSide + side;
         const float e = __shfl_sync(0xffffffffu, w, j & 31);
         if (j < cnt) {
+          const float ed = e * kJoinDown;
           sum += e;
-          acc.x = fmaf(e, v[u].x, acc.x);
-          acc.y = fmaf(e, v[u].y, acc.y);
-          acc.z = fmaf(e, v[u].z, acc.z);
-          acc.w = fmaf(e, v[u].w, acc.w);
+          acc.x = fmaf(ed, v[u].x, acc.x);
+          acc.y = fmaf(ed, v[u].y, acc.y);
+          acc.z = fmaf(ed, v[u].z, acc.z);
+          acc.w = fmaf(ed, v[u].w, acc.w);
         }
       }
     }
@@ -822,7 +831,8 @@ __global__ void __launch_bounds__(128) decode_fp8_join_few_kernel(const Fp8Decod
   }
   if (side == 0) {
     const float inv = 1.f / sum;
-    *reinterpret_cast<uint2*>(O) = make_uint2(f32_to_bf16x2(acc.x * inv, acc.y * inv), f32_to_bf16x2(acc.z * inv, acc.w * inv));
+    *reinterpret_cast<uint2*>(O) = make_uint2(f32_to_bf16x2(acc.x * inv * kJoinUp, acc.y * inv * kJoinUp),
+                                              f32_to_bf16x2(acc.z * inv * kJoinUp, acc.w * inv * kJoinUp));
     if (p.LSE && lane == 0) p.LSE[row] = (mx == -INFINITY ? 0.f : mx) + __logf(sum);
   }
 }
