@@ -324,9 +324,11 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
-    if (!ok && lane == 0) {
-      // Copies in flight must land before the block gives its memory back.  A stage
-      // that the other producer no longer filled stays open: the bound ends it.
+    if (lane == 0) {
+      // Copies in flight must land before the block gives its memory back, also when
+      // this producer got all its stages and the consumers have given up on one (else
+      // they wait for the same barriers, and this costs nothing).  A stage that the
+      // other producer no longer filled stays open: the bound ends it.
       for (uint32_t i = n > C::kStages ? n - C::kStages : 0; i < n; ++i)
         drain_wait(&bars.full[i % C::kStages], (i / C::kStages) & 1, kDrainNs);
     }
