@@ -132,7 +132,8 @@ BW_API int bw_gqa_decode(const void* Q, const void* K, const void* V, const int*
  *   K_cache, V_cache: bf16 [num_pages, page_size, Hkv, D] contiguous
  *   block_table: int32 [B, max_pages_per_seq]; token i of sequence b is slot
  *                i % page_size of page block_table[b][i / page_size]
- *   kv_lens: int32 [B];  Q, O, LSE as in bw_gqa_decode.
+ *   kv_lens: int32 [B];  Q, O, LSE as in bw_gqa_decode.  What the last page holds
+ *                behind the sequence is not used, whatever it is.
  * page_size: 8, 16, 32, 64 or any multiple of 64.  Workspace:
  * bw_gqa_decode_workspace_size(B, Hq, Hkv, D, min(num_pages * page_size,
  * B * max_pages_per_seq * page_size), chunk) bytes. */
@@ -283,9 +284,7 @@ BW_API int bw_rope(const void* Q, void* Q_out, const void* K, void* K_out, int d
  * slots int64 [T]: a negative one skips its token (padding); one beyond the
  * cache is skipped and reported as BW_ERR_INDEX by bw_stream_status.  The slots
  * of a call must differ: a slot written twice in one call holds a mixture.
- * page_size: 8, 16, 32, 64 or any multiple of 64.  T = 0 does nothing.
- * A bf16 cache should start as zeros: bw_gqa_decode_paged multiplies what a last
- * page holds behind its sequence by a weight of 0. */
+ * page_size: 8, 16, 32, 64 or any multiple of 64.  T = 0 does nothing. */
 BW_API int bw_kv_cache_write(const void* K, const void* V, const int64_t* k_strides, const int64_t* v_strides, int T,
                              int Hkv, int D, void* K_cache, void* V_cache, uint8_t* scales, int cache_dtype,
                              int page_size, int num_pages, const int64_t* slots, const float* cos_sin_cache,
