@@ -21,6 +21,7 @@ import torch
 from . import _ffi
 
 _SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
+_WANTS_GRADIENT = -1   # of the front end's rope: nothing was done, an argument requires gradients
 _front = None
 
 
@@ -58,6 +59,36 @@ def rope_table(length, rotary_dim, base=10000.0, scaling="none", factor=1.0, ori
     return out
 
 
+def _rows_of_16_bytes(t):
+    """A gradient as the call takes tensors: autograd hands over expanded and otherwise strided ones."""
+    if t is None or (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
+            n == 1 or (s > 0 and s * t.element_size() % 16 == 0) for n, s in zip(t.shape[:-1], t.stride()))):
+        return t
+    return t.contiguous()
+
+
+class _Rope(torch.autograd.Function):
+    """The rotation with its gradient, the inverse rotation of the outputs' gradients."""
+
+    @staticmethod
+    def forward(ctx, q, k, cos_sin_cache, positions, pos_offset, interleaved, inverse):
+        ctx.save_for_backward(cos_sin_cache, positions)
+        ctx.how = pos_offset, interleaved, inverse
+        ctx.set_materialize_grads(False)
+        return rope(q, k, cos_sin_cache, positions, pos_offset, interleaved, inverse)   # gradients are off here
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        (table, positions), (pos_offset, interleaved, inverse) = ctx.saved_tensors, ctx.how
+        dq, dk = _rows_of_16_bytes(dq), _rows_of_16_bytes(dk)
+        turn = lambda a, b: rope(a, b, table, positions, pos_offset, interleaved, not inverse)  # noqa: E731
+        if dq is not None:
+            dq, dk = turn(dq, dk)
+        elif dk is not None:
+            dk, _ = turn(dk, None)
+        return dq, dk, None, None, None, None, None
+
+
 def rope(q, k, cos_sin_cache, positions=None, pos_offset=0, interleaved=False, inverse=False, q_out=None, k_out=None):
     """Rotates the first cos_sin_cache.shape[1] elements of every head of q and k
     (one launch; k may be None) -> (q_out, k_out).
@@ -67,13 +98,23 @@ def rope(q, k, cos_sin_cache, positions=None, pos_offset=0, interleaved=False, i
     0, 1, ... along S.  A token whose position + pos_offset is outside the table
     is copied.  interleaved: pairs (2i, 2i + 1) instead of (i, i + R / 2).
     inverse: the transposed rotation, which maps gradients of the outputs to
-    gradients of the inputs.  q_out may be q (in place)."""
+    gradients of the inputs.  q_out may be q (in place).
+
+    Differentiable in q and k; given outputs, and a table that requires gradients,
+    are refused then."""
+    given = q_out is not None or k_out is not None
     if q_out is None:
         q_out = torch.empty_like(q)
     if k_out is None and k is not None:
         k_out = torch.empty_like(k)
     rc = (_front or _load()).rope(q, q_out, k, k_out, cos_sin_cache, positions, pos_offset, interleaved, inverse)
     if rc:
+        if rc == _WANTS_GRADIENT:
+            if cos_sin_cache.requires_grad:
+                raise ValueError("no gradient is computed for cos_sin_cache")
+            if given:
+                raise ValueError("gradients do not pass through given outputs: leave q_out and k_out out, or call under no_grad")
+            return _Rope.apply(q, k, cos_sin_cache, positions, pos_offset, interleaved, inverse)
         _ffi.check(rc, "bw_rope")
     return q_out, k_out
 

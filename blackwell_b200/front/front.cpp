@@ -13,6 +13,7 @@
 
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <ATen/core/grad_mode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/bw_attn.h"
@@ -129,11 +130,18 @@ void bhs(const char* name, const Tensor& t, bool one_sequence, int64_t* st) {
   st[2] = n == 4 ? t.stride(2) : one_sequence ? t.stride(0) : 0;
 }
 
+// Status of rope where gradients are on and an argument requires them: the call is
+// left to the caller's autograd function.  No status of the C ABI is negative.
+constexpr int kWantsGradient = -1;
+
 // rope(q, q_out, k, k_out, cos_sin_cache, positions, pos_offset, interleaved, inverse)
 int rope(PyObject* const* a) {
   const Tensor *q = tensor(a[0], "q"), *q_out = tensor(a[1], "q_out"), *k = tensor(a[2], "k", true),
                *k_out = tensor(a[3], "k_out", true), *table = tensor(a[4], "cos_sin_cache"),
                *positions = tensor(a[5], "positions", true);
+  if (at::GradMode::is_enabled())
+    for (const Tensor* t : {q, k, table, q_out, k_out})
+      if (t && t->requires_grad()) return kWantsGradient;
   const int64_t nd = q->dim();
   if (nd != 3 && nd != 4) refuse(PyExc_ValueError, "q must be [B, H, S, D] or [tokens, H, D], got " + shape_of(*q));
   const auto dtype = q->scalar_type();
