@@ -173,6 +173,7 @@ int rope(PyObject* const* a) {
     if (nd == 4) want("positions", *positions, at::kInt, {B, S});
     else want("positions", *positions, at::kInt, {B});
   }
+  if (q->numel() == 0 && k && k->numel() != 0) refuse(PyExc_ValueError, "q has no heads: give the tensor that has as q");
   void* stream = stream_for({q, k, table, positions, q_out, k_out});
   if (q->numel() == 0) return BW_OK;
   return bw_rope(ptr(q), ptr(q_out), ptr(k), ptr(k_out), dtype == at::kBFloat16 ? BW_BF16 : BW_F32, small("B", B),
