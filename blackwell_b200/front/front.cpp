@@ -279,6 +279,7 @@ int gqa_decode_paged_fp8(PyObject* const* a) {
   if (!ws->is_contiguous()) refuse(PyExc_ValueError, "workspace must be contiguous");
   const double scale = real(a[6]);
   void* stream = stream_for({q, kc, vc, scales, bt, lens, ws, out, lse});
+  if (B == 0) return BW_OK;   // no sequence
   return bw_gqa_decode_paged_fp8(ptr(q), ptr(kc), ptr(vc), static_cast<const uint8_t*>(ptr(scales)),
                                  static_cast<const int*>(ptr(bt)), static_cast<const int*>(ptr(lens)), ptr(out),
                                  static_cast<float*>(ptr(lse)), small("B", B), small("Hq", Hq), c.Hkv, c.D, c.page_size,
