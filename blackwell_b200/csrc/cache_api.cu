@@ -135,6 +135,7 @@ int bw_rope(const void* Q, void* Q_out, const void* K, void* K_out, int dtype, i
   if (!K != !K_out) return BW_ERR_NULL;
   if (dtype != BW_BF16 && dtype != BW_F32) return BW_ERR_SHAPE;
   if (B <= 0 || Hq <= 0 || S <= 0 || (K ? Hkv <= 0 : Hkv != 0) || Hq > 65536 || Hkv > 65536) return BW_ERR_SHAPE;
+  if ((Hq + 1) / 2 + (Hkv + 1) / 2 > 65535) return BW_ERR_SHAPE;   // groups of two heads along a grid's axis
   if (D <= 0 || D % 8 || D > bw::kMaxRotaryDim || rotary_dim < 16 || rotary_dim % 16 || rotary_dim > D)
     return BW_ERR_SHAPE;
   if (cache_seq_len < 0 || (int64_t)B * S >= (int64_t(1) << 31)) return BW_ERR_SHAPE;

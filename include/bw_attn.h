@@ -263,7 +263,8 @@ BW_API int bw_rope_table(float* table, int64_t length, int rotary_dim, int64_t f
  * Q_out may be Q with the same strides (in place), otherwise the two must not
  * overlap; the same for K.  Strides: elements of the (b, h, s) axes, NULL =
  * contiguous, multiples of 16 bytes.  D: a multiple of 8, at most 512;
- * rotary_dim: a multiple of 16. */
+ * rotary_dim: a multiple of 16.  Hq, Hkv: at most 65536, in pairs of heads at most
+ * 65535 together. */
 BW_API int bw_rope(const void* Q, void* Q_out, const void* K, void* K_out, int dtype, int B, int Hq, int Hkv, int S,
                    int D, const int64_t* q_strides, const int64_t* q_out_strides, const int64_t* k_strides,
                    const int64_t* k_out_strides, const float* cos_sin_cache, int64_t cache_seq_len, int rotary_dim,
