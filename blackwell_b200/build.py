@@ -4,7 +4,8 @@
 
 It also links the C++ harness ``bw_harness`` (harness/bw_harness.cpp) and the
 torch front end of the cache calls ``_front.so`` (front/front.cpp, a CPython
-module) against the library.  Every .cu under csrc/ is compiled with
+module; left out where torch's or Python's headers are missing) against the
+library.  Every .cu under csrc/ is compiled with
 ``-gencode arch=compute_100a,code=sm_100a -lineinfo -O3`` and linked into one
 shared library with the CUDA runtime linked statically (no torch types cross
 the boundary; the library only depends on the driver at run time).
@@ -12,8 +13,10 @@ the boundary; the library only depends on the driver at run time).
 from __future__ import annotations
 
 import os
+import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -39,9 +42,10 @@ def _deps():
 
 
 def up_to_date() -> bool:
-    if not OUT.exists() or not HARNESS.exists() or not FRONT.exists():
+    built = [OUT, HARNESS] if front_lacks() else [OUT, HARNESS, FRONT]
+    if not all(p.exists() for p in built):
         return False
-    t = min(OUT.stat().st_mtime, HARNESS.stat().st_mtime, FRONT.stat().st_mtime)
+    t = min(p.stat().st_mtime for p in built)
     return all(p.stat().st_mtime <= t for p in _deps() + [HARNESS_SRC, FRONT_SRC])
 
 
@@ -69,11 +73,28 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     return OUT
 
 
-def build_front(verbose: bool = False) -> Path:
-    """The torch front end: a CPython module over the C ABI, linked to the library."""
-    import shutil
-    import sysconfig
+def front_lacks():
+    """What the torch front end cannot be built without and is not here, or None."""
+    try:
+        import torch
+    except ImportError:
+        return "torch"
+    for what, there in (("g++", shutil.which("g++")),
+                        ("Python.h", (Path(sysconfig.get_paths()["include"]) / "Python.h").exists()),
+                        ("torch's headers", (Path(torch.__file__).resolve().parent / "include" / "ATen").is_dir())):
+        if not there:
+            return what
+    return None
 
+
+def build_front(verbose: bool = False):
+    """The torch front end: a CPython module over the C ABI, linked to the library.
+    Where the box has no headers for it, it is left out (the calls of cache.py say
+    so when they are used); the library and the harness do not need it."""
+    lacks = front_lacks()
+    if lacks:
+        print(f"{FRONT.name} is not built: {lacks} not found", file=sys.stderr)
+        return None
     import torch
     cuda = Path(shutil.which(NVCC) or NVCC).resolve().parent.parent
     root = Path(torch.__file__).resolve().parent
