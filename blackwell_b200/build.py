@@ -45,6 +45,8 @@ def up_to_date() -> bool:
     built = [OUT, HARNESS] if front_lacks() else [OUT, HARNESS, FRONT]
     if not all(p.exists() for p in built):
         return False
+    if FRONT in built and not front_fits():
+        return False
     t = min(p.stat().st_mtime for p in built)
     return all(p.stat().st_mtime <= t for p in _deps() + [HARNESS_SRC, FRONT_SRC])
 
@@ -87,6 +89,12 @@ def front_lacks():
     return None
 
 
+def front_fits() -> bool:
+    """Whether the torch front end was built with this torch (its version stands in the file)."""
+    import torch
+    return torch.__version__.encode() + b"\0" in FRONT.read_bytes()
+
+
 def build_front(verbose: bool = False):
     """The torch front end: a CPython module over the C ABI, linked to the library.
     Where the box has no headers for it, it is left out (the calls of cache.py say
@@ -100,7 +108,7 @@ def build_front(verbose: bool = False):
     root = Path(torch.__file__).resolve().parent
     tmp = FRONT.with_suffix(".so.tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DBW_FRONT_TORCH="{torch.__version__}"']
     for p in (root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
               cuda / "include", sysconfig.get_paths()["include"]):
         cmd += ["-isystem", str(p)]

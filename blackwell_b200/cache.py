@@ -33,7 +33,11 @@ def _load():
             raise RuntimeError(f"native front end missing: {_ffi.FRONT_PATH} "
                                "(build it with `python -m blackwell_b200.build`)")
         _ffi.lib()
-        _front = importlib.import_module("blackwell_b200._front")
+        front = importlib.import_module("blackwell_b200._front")
+        if front.built_with_torch != torch.__version__:
+            raise RuntimeError(f"{_ffi.FRONT_PATH} was built with torch {front.built_with_torch}, this is "
+                               f"{torch.__version__} (build it again with `python -m blackwell_b200.build`)")
+        _front = front
     return _front
 
 

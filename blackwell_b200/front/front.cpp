@@ -312,4 +312,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_front", "Checked calls of the rot
 
 }  // namespace
 
-extern "C" __attribute__((visibility("default"))) PyObject* PyInit__front() { return PyModule_Create(&module); }
+// BW_FRONT_TORCH: the torch version of the build (its C++ types are not another version's).
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit__front() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "built_with_torch", BW_FRONT_TORCH) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

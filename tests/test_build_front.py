@@ -33,3 +33,17 @@ def test_up_to_date_wants_the_front_where_it_can_be_built(monkeypatch, tmp_path)
         monkeypatch.setattr(build, p, tmp_path / p)
     monkeypatch.setattr(build, "FRONT", tmp_path / "_front.so")
     assert build.front_lacks() is None and not build.up_to_date()
+
+
+def test_front_of_another_torch_is_noticed(monkeypatch):
+    """By the build, which makes it again, and by the first call, which says so."""
+    import torch
+
+    import blackwell_b200 as bw
+    from blackwell_b200 import cache
+    assert build.front_fits()
+    monkeypatch.setattr(torch, "__version__", "1.0.0")
+    assert not build.front_fits() and not build.up_to_date()
+    monkeypatch.setattr(cache, "_front", None)
+    with pytest.raises(RuntimeError, match="built with torch"):
+        bw.rope(torch.zeros(3, 4, 64), None, torch.zeros(8, 64))
