@@ -241,10 +241,12 @@ __global__ void __launch_bounds__(kThreads)
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
     }
-    if (!ok && lane == 0) {
-      // unwinding: wait for the loads already in flight before exiting
+    if (lane == 0) {
+      // Loads in flight land before the block gives its memory back, also when the
+      // producer got all its stages and the consumers have given up on one (else they
+      // wait for the same barriers, and this costs nothing).
       for (uint32_t i = n > kStages ? n - kStages : 0; i < n; ++i)
-        drain_wait(&bars.full[i % kStages], (i / kStages) & 1, p.timeout_ns);
+        drain_wait(&bars.full[i % kStages], (i / kStages) & 1, kDrainNs);
     }
     return;
   }

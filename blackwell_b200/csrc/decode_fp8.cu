@@ -53,7 +53,6 @@ constexpr int kStep = 64;   // tokens of a step: 16 a consumer warp
 __host__ __device__ constexpr int tile_steps(int D) { return D == 128 ? 2 : 4; }
 __host__ __device__ constexpr int tile_tokens(int D) { return kStep * tile_steps(D); }
 constexpr int kMaxB = 4096;
-constexpr uint64_t kDrainNs = 20000000;   // 20 ms, thousands of times what a copy takes
 constexpr int kWarps = 4;      // consumers; one producer warp more for K and one for V
 constexpr int kThreads = 32 * (kWarps + 2);
 // Resident blocks an SM: 97 KB of stages and up to 168 registers a thread each.

@@ -122,6 +122,8 @@ __device__ __forceinline__ bool spin_wait(const WaitCtl& wc, uint64_t* bar, uint
   }
 }
 
+constexpr uint64_t kDrainNs = 20000000;   // bound on copies in flight: 20 ms, thousands of times what one takes
+
 // Bounded wait used while unwinding after an abort: ignores the abort flag so
 // that copies and MMAs already in flight are waited for before TMEM and shared
 // memory are released.
