@@ -44,6 +44,7 @@ struct DecCfg {
 struct DecBars {
   uint64_t full[kStages], empty[kStages];
   int abort_flag;
+  int stop;   // what the consumers make of abort_flag at the end of an item
   int total_parts;
   long long warp_sum[kThreads / 32];
 };
@@ -294,7 +295,8 @@ __global__ void __launch_bounds__(kThreads)
       const uint32_t s = n % kStages;
       // On a timeout the warp still runs this item's merge below, so that the
       // named barriers stay matched across the consumer warps, then stops.
-      if (!wc.wait(&bars.full[s], (n / kStages) & 1)) { ok = false; break; }
+      const bool got = wc.wait(&bars.full[s], (n / kStages) & 1);
+      if (!__all_sync(0xffffffffu, got)) break;   // the warp decides as one
       const int64_t tw = t + warp * 16;         // first token of this warp's slice
       if (tw < it.t1) {
         const uint32_t kb = sbase + s * C::kStage;
@@ -425,8 +427,10 @@ __global__ void __launch_bounds__(kThreads)
       acc[i] = 0.f;
       if ((i % D) == 0) p.lse_part[(int64_t)it.part * p.G + row] = (M + __log2f(Ls)) * 0.69314718055994531f;
     }
+    if (tid == 0) bars.stop = *wc.abort_flag;
     consumer_sync();
-    if (*wc.abort_flag) ok = false;
+    // All warps stop at the same item, so that none waits at a barrier for one that has left.
+    if (*(volatile int*)&bars.stop) ok = false;
   }
 }
 
