@@ -24,14 +24,17 @@
 //
 // Measured on B200 (device time; share of the 6.45 TB/s that a copy reaches):
 //   64 sequences of 1024 to 32768 tokens, 8 KV heads, G = 8, D = 128
-//     pages of 64   326 - 356 us   97 - 106 %   (by box; the bf16 cache has twice the bytes)
+//     pages of 64   329 - 356 us   97 - 105 %   (by box; the bf16 cache has twice the bytes)
 //     pages of 16   335 us         103 %
 //     pages of 8    390 us          88 %         one tensor copy per 8 rows
 //     D = 64        179 us          97 %
-//   32 sequences of 1000 to 32768, 4 KV heads, G = 16: 103 us, 84 %: two products
-//     and softmaxes a code, 8 consumer warps an SM hide their latency no further
-//   1 sequence of 131072: 49 us, 85 %: start, last merge and join take 7
-//   1 sequence of 517: 7.3 us: launch 0.4, tile counts 1, page index and first tile
+//   32 sequences of 1000 to 32768, 4 KV heads, G = 16: 104 us, 83 %: two products
+//     and softmaxes a code on the same 8 consumer warps an SM.  They issue in 50 % of
+//     the cycles (G = 8: 42 %) and wait for memory a quarter as long (0.5 against 2.0
+//     warps an issue): what bounds them is the latency of their own instructions, and
+//     168 registers leave no room to start the next tile under it
+//   1 sequence of 131072: 50 us, 84 %: start, last merge and join take 7
+//   1 sequence of 517: 7.5 us: launch 0.4, tile counts 1, page index and first tile
 //     2.1, products 0.8, merge 0.9, join 2
 #include <cuda_bf16.h>
 
@@ -225,6 +228,14 @@ __device__ __forceinline__ Segment next_segment(const Fp8DecodeParams& p, const 
 // The denominator has its own reference m (the maximum of x): one more ex2 an
 // element.  Both references follow their maximum only when it has moved by more
 // than 2^8; m is per thread, M per warp (votes; shuffles only when it moves).
+// A value row of zeros has no part in M (see there).
+//
+// Rounded to fewer bits than 32: Q to f16 (nothing down to 2^-14 of its row's
+// largest) and the weight to f16 (2^-11 of itself; the bf16 decode's are bf16,
+// 2^-8), since the product wants both as the codes are.  Sums, the denominator and
+// the references are fp32.  Against 64 bits the output is as far off as one from
+// fp32 weights (1.6e-3 of its norm, the rounding to bf16); the two differ by single
+// bf16 steps (1.4e-4 to 6.5e-4 of the norm).
 //
 // WHOLE: runs begin and end with a sequence, so that none is cut and no join follows.
 template <int D, int NT, bool WHOLE>
@@ -465,7 +476,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
             const int u = e / 2, i = e % 2;
             float a = acc[u][nt][0][2 * i + j];
             if constexpr (kChains == 2) a += acc[u][nt][1][2 * i + j];
-            // Key and query scales may be far out and make up for each other: a small qs goes to ks first, a large one last.
+            // Key and query scales may be far out and make up for each other: a small qs goes to ks first, a
+            // large one last (a third product an element: up to 1 % of the time).
             x[j][e] = a * (ks[u][i] * fminf(qs[nt][j], 1.f)) * fmaxf(qs[nt][j], 1.f);
           }
         if (some) {
@@ -856,12 +868,15 @@ cudaError_t launch_main(const Fp8DecodeParams& p, const Fp8DecodeMaps& maps, cud
 
 template <int D, int NT>
 cudaError_t launch(const Fp8DecodeParams& p, const Fp8DecodeMaps& maps, cudaStream_t stream) {
-  // Sequences of a few tiles (by the table's width) are not cut: the join and its
-  // launch would cost more than a block's further tiles.  Up to two tiles always
-  // (48 sequences of up to 107 tokens, 4 KV heads, D = 64: 8.0 -> 6.8 us), up to
-  // four where sequences and heads occupy the GPU (16 of up to 500 tokens, 8 KV
-  // heads: 10.8 -> 9.4; 2 of up to 1000, 2 KV heads, D = 64: 8.0 cut, 8.9 not).
-  // With up to eight it is slower or the same (16 of up to 1000: 12.0 cut, 13.5 not).
+  // Sequences of a few tiles are not cut: the join and its launch would cost more
+  // than a block's further tiles.  The table's width decides, which is all that the
+  // host knows of the lengths: a table of fixed width gets the cut and the join for
+  // the same sequences.  Up to two tiles always (48 sequences of up to 107 tokens, 4
+  // KV heads, D = 64: 6.1 us; with a table for 131072 tokens 7.0), up to four where
+  // sequences and heads occupy the GPU (16 of up to 500 tokens, 8 KV heads: 9.9, 10.8;
+  // 116 of up to 246: 18.8, 20.4; but 2 of up to 1000, 2 KV heads, D = 64: 8.9 not cut,
+  // 8.0 cut).  With up to eight it is slower or the same (16 of up to 1000: 13.5 not
+  // cut, 12.0 cut).
   const int tiles = (p.max_tokens + Cfg<D>::kTile - 1) / Cfg<D>::kTile;
   if (tiles <= 2 || (tiles <= 4 && 4 * p.B >= p.groups)) return launch_main<D, NT, true>(p, maps, stream);
   const cudaError_t e = launch_main<D, NT, false>(p, maps, stream);

@@ -25,7 +25,9 @@ namespace {
 // so positions of millions keep full fp32 accuracy; the rest, at most half a
 // quarter turn, goes to fp32.  Adding 1.5 * 2^52 rounds to a whole number whose
 // low bits are the quadrant, which saves the conversions between fp64 and
-// integers.  Bound by the stores.
+// integers.  The series and the product with the magnitude are fp32, as the table
+// is (3.5e-8 of the result off at 131072 rows with YaRN, an fp64 series rounded
+// once 2.7e-8): fp64 would be the bound instead of the stores.
 constexpr int kTableThreads = 256, kTableBlocks = 6;   // resident blocks an SM, by registers
 
 __global__ void __launch_bounds__(kTableThreads, kTableBlocks) rope_table_kernel(const RopeTableParams p) {
@@ -153,9 +155,10 @@ cudaError_t launch(RopeParams p, unsigned token_blocks, cudaStream_t stream) {
 }
 
 // Four heads a thread re-use its angles and keep eight loads in flight; where that
-// leaves less than a wave of blocks, two heads spread the work (2960 x 3 tokens, 8
-// heads of 80: 5.1 -> 4.8 us; 1777 x 3 tokens, 16 heads of 64 in fp32, more than a
-// wave: 8.8 us with four heads, 9.6 with two; 4 x 4096 tokens, 40 heads: 54.8, 55.3).
+// leaves less than a wave of blocks, two heads spread the work (2960 x 3 tokens, 6 + 2
+// heads of 80: 4.8 -> 4.5 us, 7 + 1 heads 4.8 -> 5.1; 1777 x 3 tokens, 12 + 4 heads of
+// 64 in fp32, more than a wave: 8.7 us with four heads, 9.4 with two; 4 x 4096 tokens,
+// 40 heads: 55.3, 57.8).
 template <typename T>
 cudaError_t launch_heads(RopeParams p, int num_sms, cudaStream_t stream) {
   p.block_tokens = kRopeThreads / p.units;   // units: at most 64
