@@ -151,10 +151,9 @@ __device__ void x3_producer(const F32x3Params& p, const F32x3Maps& maps, uint8_t
       tma_load_4d(smem + kOffQ + part * kQTile + c * kQPanel, part ? &maps.q_lo : &maps.q_hi, &bars.q_full, c * 32,
                   it.qt * kRows, it.h, it.b);
   int j = 0;
-  bool ok = true;
   for (; j < n; ++j) {
     const int st = j % kNS;
-    if (!wc.wait(&bars.kv_empty[st], ((j / kNS) & 1) ^ 1)) { ok = false; break; }
+    if (!wc.wait(&bars.kv_empty[st], ((j / kNS) & 1) ^ 1)) break;
     mbar_arrive_expect_tx(&bars.kv_full[st], kStage);
     uint8_t* dst = smem + kOffKV + st * kStage;
     for (int part = 0; part < 2; ++part) {
@@ -165,11 +164,10 @@ __device__ void x3_producer(const F32x3Params& p, const F32x3Maps& maps, uint8_t
                   0, it.h, it.b);
     }
   }
-  if (!ok) {
-    // unwinding: wait for the loads already issued before the CTA exits
-    for (int i = j > kNS ? j - kNS : 0; i < j; ++i) drain_wait(&bars.kv_full[i % kNS], (i / kNS) & 1, wc.timeout_ns);
-    drain_wait(&bars.q_full, 0, wc.timeout_ns);
-  }
+  // Loads in flight land before the block gives its memory back, also when every
+  // load was issued and the consumers have given up on one.
+  for (int i = j > kNS ? j - kNS : 0; i < j; ++i) drain_wait(&bars.kv_full[i % kNS], (i / kNS) & 1, kDrainNs);
+  drain_wait(&bars.q_full, 0, kDrainNs);
 }
 
 __device__ void x3_mma(const F32x3Params& p, uint8_t* smem, BarsX3& bars, const WaitCtl& wc, uint32_t tmem) {
@@ -225,7 +223,7 @@ __device__ void x3_mma(const F32x3Params& p, uint8_t* smem, BarsX3& bars, const 
     tc_commit(&bars.kv_empty[j % kNS]);
   }
   tc_commit(&bars.mma_done);
-  drain_wait(&bars.mma_done, 0, wc.timeout_ns);
+  drain_wait(&bars.mma_done, 0, kDrainNs);
 }
 
 __device__ void x3_softmax(const F32x3Params& p, uint8_t* smem, BarsX3& bars, const WaitCtl& wc, uint32_t tmem,

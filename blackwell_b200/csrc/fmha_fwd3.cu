@@ -193,13 +193,14 @@ __device__ void producer3(const FmhaParams& p, const FmhaMaps& maps, uint8_t* sm
       }
     }
   }
-  if (!ok) {
-    for (uint32_t i = (ld > NS ? ld - NS : 0); i < ld; ++i) {
-      const uint32_t slot = i % NS;
-      if (armed & (1u << slot)) drain_wait(&bars.kv_full[slot], (i / NS) & 1, wc.timeout_ns);
-    }
-    for (uint32_t i = qn > 2 ? qn - 2 : 0; i < qn; ++i) drain_wait(&bars.q_full[i & 1], (i >> 1) & 1, wc.timeout_ns);
+  // Loads in flight land before the block gives its memory back, also when every
+  // load was issued and the consumers have given up on one (else they wait for the
+  // same barriers, and this costs nothing).
+  for (uint32_t i = (ld > NS ? ld - NS : 0); i < ld; ++i) {
+    const uint32_t slot = i % NS;
+    if (armed & (1u << slot)) drain_wait(&bars.kv_full[slot], (i / NS) & 1, kDrainNs);
   }
+  for (uint32_t i = qn > 2 ? qn - 2 : 0; i < qn; ++i) drain_wait(&bars.q_full[i & 1], (i >> 1) & 1, kDrainNs);
 }
 
 // ---------------------------------------------------------------- MMA warps
@@ -272,7 +273,7 @@ __device__ void qk_issuer3(const FmhaParams& p, uint8_t* smem, Bars3& bars, cons
     }
   }
   tc_commit(&bars.qk_done);
-  drain_wait(&bars.qk_done, 0, wc.timeout_ns);
+  drain_wait(&bars.qk_done, 0, kDrainNs);
 }
 
 template <int D, int V>
@@ -326,7 +327,7 @@ __device__ void pv_issuer3(const FmhaParams& p, uint8_t* smem, Bars3& bars, cons
     }
   }
   tc_commit(&bars.mma_done);
-  drain_wait(&bars.mma_done, 0, wc.timeout_ns);
+  drain_wait(&bars.mma_done, 0, kDrainNs);
 }
 
 __device__ __forceinline__ uint32_t pack_bf16_3(float lo, float hi) {

@@ -124,9 +124,9 @@ __device__ __forceinline__ bool spin_wait(const WaitCtl& wc, uint64_t* bar, uint
 
 constexpr uint64_t kDrainNs = 20000000;   // bound on copies in flight: 20 ms, thousands of times what one takes
 
-// Bounded wait used while unwinding after an abort: ignores the abort flag so
-// that copies and MMAs already in flight are waited for before TMEM and shared
-// memory are released.
+// Bounded wait before a role leaves: ignores the abort flag, and the bound on waits
+// that a user may have set to less than a copy takes, so that copies and MMAs
+// already in flight are waited for before TMEM and shared memory are released.
 __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity, uint64_t timeout_ns) {
   const uint64_t t0 = globaltimer_ns();
   while (!mbar_try_wait(bar, parity)) {
